@@ -328,6 +328,60 @@ int int8kv_static_ws_status(void* dst, int clear, void* stream);
 int int8kv_static_ws_address(void** device_ptr);
 
 /*
+ * Block tables and slot maps from request lengths, on the device (no counterpart in the reference, whose tests and
+ * engine build both on the host).  A block is `block_size` (S) consecutive tokens of one request; row b of
+ * block_tables [num_requests, bt_width] lists its physical blocks.  Free blocks are a list with a cursor:
+ * free_blocks[*free_cursor .. num_free) are free, the entries below the cursor have been handed out.
+ *
+ * int8kv_build_block_tables: request b holds seq_lens[b] tokens and gets new_lens[b] more (negative values count as 0).
+ * Requests take the blocks they lack, ceil((c + n) / S) - ceil(c / S), from the cursor on, in request order, and
+ * their rows are extended in place; nothing else of the table is written.  A request whose tokens do not fit its
+ * table row, or for which the free list has not enough left, is refused: it gets no block, its length stays, its
+ * tokens get slot -1, and so does every later request that needs a block once the list ran out (a refusal by the
+ * row's width takes nothing from the list).  Outputs:
+ *   slot_mapping [num_tokens]  int64: the new tokens of all requests packed in request order, token i of request b at
+ *                query_start[b] + i, slot = block * S + offset; -1 for refused tokens, for blocks with a negative id
+ *                and behind the last token.  num_tokens (below 2^31) should be at least the sum of new_lens; what
+ *                lies beyond it gets its blocks but no slot
+ *   query_start  [num_requests + 1] int32: exclusive prefix sums of new_lens
+ *   seq_lens_out [num_requests], the type of seq_lens: lengths after the step (the old one where refused)
+ *   free_cursor_out: the cursor behind the last block taken
+ * seq_lens_out may be seq_lens and free_cursor_out may be free_cursor: a captured step then advances its own state.
+ * int8kv_build_slot_mapping: the slots and prefix sums alone, through tables that already hold the blocks of the new
+ * tokens (-1 beyond the row).
+ * int8kv_release_block_tables: the blocks of the requests with finished[b] != 0 (ceil(seq_lens[b] / S) entries of their
+ * rows, seq_lens clamped to what a row holds) go back below the cursor, in request order, and their lengths become 0;
+ * the table is not written.  Entries that would lie below position 0 (more blocks given back than were handed out) are
+ * dropped.  In-place outputs as above.
+ * workspace: int8kv_block_tables_workspace_bytes(num_requests, items) bytes, 16-byte aligned; 0 (and a null workspace)
+ * for calls that run as one kernel.  items is an upper bound of the slots and blocks a call writes: num_tokens +
+ * num_tokens / S + num_requests for a growth, num_tokens for a slot mapping, min(num_requests * bt_width, num_free)
+ * for a release.
+ */
+int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items);
+
+int int8kv_build_block_tables(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
+                              int num_requests, int block_size,
+                              void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
+                              const void* free_blocks, int fb_is_i64, int64_t num_free,
+                              const int64_t* free_cursor, int64_t* free_cursor_out, void* seq_lens_out,
+                              int64_t* slot_mapping, int64_t num_tokens, int32_t* query_start,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+int int8kv_build_slot_mapping(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
+                              int num_requests, int block_size,
+                              const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
+                              int64_t* slot_mapping, int64_t num_tokens, int32_t* query_start,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+int int8kv_release_block_tables(const void* seq_lens, int sl_is_i64, const uint8_t* finished,
+                                int num_requests, int block_size,
+                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
+                                void* free_blocks, int fb_is_i64, int64_t num_free,
+                                const int64_t* free_cursor, int64_t* free_cursor_out, void* seq_lens_out,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Merge `num_parts` partial results.  Replaces _merge_split_kv_kernel (reference
  * src/triton_ops/int8_paged_attention.py:330-388): out = sum_r w_r * out_r / sum_r w_r, w_r = exp(lse_r - max lse);
  * parts with lse = -inf are ignored; all-empty rows give zeros.  `parts` is [num_parts, rows, row_floats] fp32 with

@@ -4,6 +4,7 @@ interface of the research prototype cjsmt/Int8-kvcache.
 The directory name contains a hyphen, so import it with
 `importlib.import_module("int8-kvcache_b200")`; sub-modules use relative imports.
 
+    block_tables   build_block_tables / build_slot_mapping / release_block_tables
     ops            int8_kv_cache_write / int8_paged_attention / bf16_paged_attention (+ partial/merge)
     triton_ops/    drop-in modules with the reference's module and function names
     vllm_int8/     drop-in cache-ops, cache-pool and attention call-site modules
@@ -13,6 +14,12 @@ The directory name contains a hyphen, so import it with
 """
 
 from . import _lib  # noqa: F401
+from .block_tables import (  # noqa: F401
+    BlockTableStep,
+    build_block_tables,
+    build_slot_mapping,
+    release_block_tables,
+)
 from .ops import (  # noqa: F401
     bf16_paged_attention,
     device_status,
@@ -45,6 +52,10 @@ __all__ = [
     "int8_decode_step_layers",
     "DecodeStepLayers",
     "reshape_and_cache_int8",
+    "BlockTableStep",
+    "build_block_tables",
+    "build_slot_mapping",
+    "release_block_tables",
     "merge_partials",
     "partial_row_floats",
     "device_status",

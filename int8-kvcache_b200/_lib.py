@@ -121,6 +121,22 @@ _SIGNATURES = {
          _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64, C.c_int, _I64P,
          C.c_int, _VP, C.c_int64, C.c_int, _VP],
     ),
+    "int8kv_block_tables_workspace_bytes": (C.c_int64, [C.c_int, C.c_int64]),
+    "int8kv_build_block_tables": (
+        C.c_int,
+        [_VP, C.c_int, _VP, C.c_int, C.c_int, C.c_int, _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64,
+         _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP, C.c_int64, _VP],
+    ),
+    "int8kv_build_slot_mapping": (
+        C.c_int,
+        [_VP, C.c_int, _VP, C.c_int, C.c_int, C.c_int, _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int64, _VP,
+         _VP, C.c_int64, _VP],
+    ),
+    "int8kv_release_block_tables": (
+        C.c_int,
+        [_VP, C.c_int, _VP, C.c_int, C.c_int, _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64,
+         _VP, _VP, _VP, _VP, C.c_int64, _VP],
+    ),
     "int8kv_static_ws_status": (C.c_int, [_VP, C.c_int, _VP]),
     "int8kv_static_ws_address": (C.c_int, [C.POINTER(_VP)]),
     "int8kv_exchange_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int, C.c_int]),

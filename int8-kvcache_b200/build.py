@@ -18,7 +18,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libint8kv_b200.so"
-SOURCES = ["c_api.cu", "cache_write.cu", "paged_attn.cu"]
+SOURCES = ["c_api.cu", "cache_write.cu", "paged_attn.cu", "block_tables.cu"]
 HEADERS = ["common.cuh", "kernels.h", "../../include/int8kv_b200.h"]
 
 NVCC_FLAGS = [
@@ -27,6 +27,8 @@ NVCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-lineinfo",
+    "--threads",
+    "0",
     "--shared",
     "-Xcompiler",
     "-fPIC",

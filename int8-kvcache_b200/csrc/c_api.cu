@@ -989,3 +989,96 @@ int int8kv_static_ws_status(void* dst, int clear, void* stream) {
 }
 
 }  // extern "C"
+
+// =============================================================================================================
+// Block tables and slot maps
+// =============================================================================================================
+namespace {
+
+constexpr int64_t kMaxIndex = (int64_t(1) << 31) - 1;  // tokens, columns and list entries are numbered in 32 bits
+
+// The arguments that the three operators share.
+int table_params(TableParams& p, int mode, const void* lens, int lens_is_i64, int R, int block_size, void* bt,
+                 int bt_is_i64, const int64_t* bt_st, int64_t width) {
+  std::memset(&p, 0, sizeof(p));
+  if (R < 0 || R >= kMaxIndex || block_size <= 0 || width < 0 || width >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
+  if (R > 0 && (!lens || !bt_st || (width > 0 && !bt))) return INT8KV_E_NULLPTR;
+  p.mode = mode;
+  p.R = R; p.block_size = block_size; p.width = width;
+  p.bt = bt; p.bt_is_i64 = bt_is_i64;
+  if (bt_st) { p.bt_st[0] = bt_st[0]; p.bt_st[1] = bt_st[1]; }
+  p.lens = lens; p.lens_is_i64 = lens_is_i64;
+  return INT8KV_OK;
+}
+
+int run_tables(const TableParams& p, int64_t items, void* ws, int64_t ws_size, void* stream) {
+  const int64_t need = table_single_launch(p.R, items) ? 0 : table_workspace_bytes(p.R);
+  if (need > 0 && (ws == nullptr || ws_size < need || (reinterpret_cast<uintptr_t>(ws) & 15u))) return INT8KV_E_WORKSPACE;
+  return launch_tables(p, ws, items, device_sm_count(), static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items) {
+  if (num_requests < 0 || items < 0) return -1;
+  return table_single_launch(num_requests, items) ? 0 : table_workspace_bytes(num_requests);
+}
+
+int int8kv_build_block_tables(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
+                              int num_requests, int block_size, void* block_tables, int bt_is_i64,
+                              const int64_t bt_strides[2], int64_t bt_width, const void* free_blocks, int fb_is_i64,
+                              int64_t num_free, const int64_t* free_cursor, int64_t* free_cursor_out,
+                              void* seq_lens_out, int64_t* slot_mapping, int64_t num_tokens, int32_t* query_start,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  TableParams p;
+  const int rc = table_params(p, kTabGrow, seq_lens, sl_is_i64, num_requests, block_size, block_tables, bt_is_i64,
+                              bt_strides, bt_width);
+  if (rc != INT8KV_OK) return rc;
+  if (num_free < 0 || num_free >= kMaxIndex || num_tokens < 0 || num_tokens >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
+  if (!free_cursor || !free_cursor_out || !query_start) return INT8KV_E_NULLPTR;
+  if ((num_requests > 0 && (!new_lens || !seq_lens_out)) || (num_free > 0 && !free_blocks) ||
+      (num_tokens > 0 && !slot_mapping))
+    return INT8KV_E_NULLPTR;
+  p.new_lens = new_lens; p.new_is_i64 = nl_is_i64; p.lens_out = seq_lens_out;
+  p.free_blocks = free_blocks; p.free_is_i64 = fb_is_i64; p.num_free = num_free;
+  p.cursor = free_cursor; p.cursor_out = free_cursor_out;
+  p.slots = slot_mapping; p.num_tokens = num_tokens; p.query_start = query_start;
+  return run_tables(p, num_tokens + num_tokens / block_size + num_requests, workspace, workspace_bytes, stream);
+}
+
+int int8kv_build_slot_mapping(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
+                              int num_requests, int block_size, const void* block_tables, int bt_is_i64,
+                              const int64_t bt_strides[2], int64_t bt_width, int64_t* slot_mapping, int64_t num_tokens,
+                              int32_t* query_start, void* workspace, int64_t workspace_bytes, void* stream) {
+  TableParams p;
+  const int rc = table_params(p, kTabSlots, seq_lens, sl_is_i64, num_requests, block_size,
+                              const_cast<void*>(block_tables), bt_is_i64, bt_strides, bt_width);
+  if (rc != INT8KV_OK) return rc;
+  if (num_tokens < 0 || num_tokens >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
+  if (!query_start || (num_requests > 0 && !new_lens) || (num_tokens > 0 && !slot_mapping)) return INT8KV_E_NULLPTR;
+  p.new_lens = new_lens; p.new_is_i64 = nl_is_i64;
+  p.slots = slot_mapping; p.num_tokens = num_tokens; p.query_start = query_start;
+  return run_tables(p, num_tokens, workspace, workspace_bytes, stream);
+}
+
+int int8kv_release_block_tables(const void* seq_lens, int sl_is_i64, const uint8_t* finished, int num_requests,
+                                int block_size, const void* block_tables, int bt_is_i64, const int64_t bt_strides[2],
+                                int64_t bt_width, void* free_blocks, int fb_is_i64, int64_t num_free,
+                                const int64_t* free_cursor, int64_t* free_cursor_out, void* seq_lens_out,
+                                void* workspace, int64_t workspace_bytes, void* stream) {
+  TableParams p;
+  const int rc = table_params(p, kTabRelease, seq_lens, sl_is_i64, num_requests, block_size,
+                              const_cast<void*>(block_tables), bt_is_i64, bt_strides, bt_width);
+  if (rc != INT8KV_OK) return rc;
+  if (num_free < 0 || num_free >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
+  if (!free_cursor || !free_cursor_out || (num_free > 0 && !free_blocks)) return INT8KV_E_NULLPTR;
+  if (num_requests > 0 && (!finished || !seq_lens_out)) return INT8KV_E_NULLPTR;
+  p.finished = finished; p.lens_out = seq_lens_out;
+  p.free_out = free_blocks; p.free_is_i64 = fb_is_i64; p.num_free = num_free;
+  p.cursor = free_cursor; p.cursor_out = free_cursor_out;
+  return run_tables(p, std::min<int64_t>(num_requests * bt_width, num_free), workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -165,6 +165,53 @@ struct ChainedMerge {
   int duty;
 };
 
+// Block tables and slot maps (block_tables.cu).
+// What the write phase needs of a request.
+struct alignas(16) TabRecord {
+  int64_t cached;   // tokens it held; -1: refused or not taking part
+  uint32_t start;   // first of its tokens in the packed order (growth, slots)
+  uint32_t first;   // first of its blocks in the order of all blocks that move
+};
+
+struct TabTotals {
+  uint32_t tokens;  // new tokens of all requests
+  uint32_t blocks;  // blocks that all requests want, or that finished requests give back
+  int64_t cursor;   // the free list's cursor before the call
+};
+
+enum TableMode { kTabGrow = 0, kTabSlots = 1, kTabRelease = 2 };
+
+struct TableParams {
+  int mode;
+  int R, block_size;
+  int64_t width;          // table columns
+  void* bt;               // [R, width]: read, and written by a growth
+  int bt_is_i64;
+  int64_t bt_st[2];
+  const void* lens;       // [R]
+  void* lens_out;         // [R], the type of lens; may be lens itself (growth, release)
+  int lens_is_i64;
+  const void* new_lens;   // [R] (growth, slots)
+  int new_is_i64;
+  const uint8_t* finished;  // [R] (release)
+  const void* free_blocks;  // [num_free] (growth reads it, release writes free_out)
+  void* free_out;
+  int free_is_i64;
+  int64_t num_free;
+  const int64_t* cursor;  // [1] (growth, release); cursor_out may be the same word
+  int64_t* cursor_out;
+  int64_t* slots;         // [num_tokens]
+  int64_t num_tokens;     // below 2^31
+  int32_t* query_start;   // [R + 1]
+  TabRecord* records;     // two-kernel form: [R] in the workspace, behind the totals
+  TabTotals* totals;
+};
+
+int64_t table_workspace_bytes(int R);
+// Whether a call of R requests with at most `items` slots and moved blocks runs as one kernel, without a workspace.
+bool table_single_launch(int R, int64_t items);
+int launch_tables(TableParams p, void* workspace, int64_t items, int sm_count, cudaStream_t stream);
+
 int launch_cache_write(const WriteParams& p, int sm_count, cudaStream_t stream);
 int launch_cache_write_dynamic(const DynWriteParams& p, cudaStream_t stream);
 // `prev`: null, or the merge of the previous layer's partial rows to be carried by this launch (tiled kernels with
