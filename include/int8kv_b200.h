@@ -328,6 +328,53 @@ int int8kv_static_ws_status(void* dst, int clear, void* stream);
 int int8kv_static_ws_address(void** device_ptr);
 
 /*
+ * Differential paged decode attention (no counterpart in the reference).  A layer of `num_heads` differential heads over
+ * `num_kv_pairs` pairs of KV heads: query [B, 2 * num_heads, D], caches [num_blocks, BS, 2 * num_kv_pairs, D] as the
+ * cache writes fill them (heads 2g and 2g + 1 of K are the keys of the two maps of pair g; heads 2g and 2g + 1 of V
+ * are the two halves of its value rows of 2 D), out [B, num_heads, 2 D].  Differential head h reads pair
+ * h / (num_heads / num_kv_pairs):
+ *   o = (softmax(q[2h] . K[2g]^T / sqrt(D)) - lam[h] * softmax(q[2h + 1] . K[2g + 1]^T / sqrt(D))) . V[2g, 2g + 1]
+ *   out = out_scale * o                                                      without norm_weight
+ *   out = out_scale * norm_weight * o / sqrt(mean(o^2) + norm_eps)           with it (mean over the 2 D values)
+ * A sequence with seq_len <= 0 yields zeros.  D <= 256.
+ *   k_scale / v_scale  [2 * num_kv_pairs] fp32 (int8 form): the scales the cache was written with
+ *   lam                [num_heads] or, with lam_stride 0, one value; lam_dtype and norm_dtype are float dtype codes
+ *   norm_weight        [2 D] contiguous, or NULL; norm_eps > 0 with it
+ *   num_splits         0 = choose from the shape, >= 1 = exactly that many (at most int8kv_max_splits())
+ *   workspace          int8kv_diff_workspace_bytes() bytes, 16-byte aligned (always needed: the maps' rows go through it)
+ *   status             device word for INT8KV_DEV_* bits, or NULL
+ */
+int64_t int8kv_diff_workspace_bytes(int batch, int num_heads, int num_kv_pairs, int head_dim, int64_t max_seq_len,
+                                    int block_size, int num_splits, int sm_count);
+
+int int8kv_paged_diff_attn_int8(const void* query, int q_dtype, const int64_t q_strides[3],
+                                int batch, int num_heads, int num_kv_pairs, int head_dim,
+                                const int8_t* key_cache, const int8_t* value_cache,
+                                const int64_t key_cache_strides[4], const int64_t value_cache_strides[4],
+                                int64_t num_blocks, int block_size,
+                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
+                                const void* seq_lens, int sl_is_i64, int64_t max_seq_len_hint,
+                                const float* k_scale, const float* v_scale,
+                                const void* lam, int lam_dtype, int64_t lam_stride,
+                                const void* norm_weight, int norm_dtype, float norm_eps, float out_scale,
+                                void* out, int out_dtype, const int64_t out_strides[3],
+                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
+                                void* stream);
+
+int int8kv_paged_diff_attn_bf16(const void* query, int q_dtype, const int64_t q_strides[3],
+                                int batch, int num_heads, int num_kv_pairs, int head_dim,
+                                const void* key_cache, const void* value_cache, int cache_dtype,
+                                const int64_t key_cache_strides[4], const int64_t value_cache_strides[4],
+                                int64_t num_blocks, int block_size,
+                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
+                                const void* seq_lens, int sl_is_i64, int64_t max_seq_len_hint,
+                                const void* lam, int lam_dtype, int64_t lam_stride,
+                                const void* norm_weight, int norm_dtype, float norm_eps, float out_scale,
+                                void* out, int out_dtype, const int64_t out_strides[3],
+                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
+                                void* stream);
+
+/*
  * Block tables and slot maps from request lengths, on the device (no counterpart in the reference, whose tests and
  * engine build both on the host).  A block is `block_size` (S) consecutive tokens of one request; row b of
  * block_tables [num_requests, bt_width] lists its physical blocks.  Free blocks are a list with a cursor:

@@ -5,6 +5,7 @@ The directory name contains a hyphen, so import it with
 `importlib.import_module("int8-kvcache_b200")`; sub-modules use relative imports.
 
     block_tables   build_block_tables / build_slot_mapping / release_block_tables
+    diff_attention int8_paged_diff_attention / bf16_paged_diff_attention
     ops            int8_kv_cache_write / int8_paged_attention / bf16_paged_attention (+ partial/merge)
     triton_ops/    drop-in modules with the reference's module and function names
     vllm_int8/     drop-in cache-ops, cache-pool and attention call-site modules
@@ -20,6 +21,7 @@ from .block_tables import (  # noqa: F401
     build_slot_mapping,
     release_block_tables,
 )
+from .diff_attention import bf16_paged_diff_attention, int8_paged_diff_attention  # noqa: F401
 from .ops import (  # noqa: F401
     bf16_paged_attention,
     device_status,
@@ -52,6 +54,8 @@ __all__ = [
     "int8_decode_step_layers",
     "DecodeStepLayers",
     "reshape_and_cache_int8",
+    "int8_paged_diff_attention",
+    "bf16_paged_diff_attention",
     "BlockTableStep",
     "build_block_tables",
     "build_slot_mapping",

@@ -1082,3 +1082,131 @@ int int8kv_release_block_tables(const void* seq_lens, int sl_is_i64, const uint8
 }
 
 }  // extern "C"
+
+// =============================================================================================================
+// Differential attention
+// =============================================================================================================
+namespace {
+
+// Split count of the kernel for every shape: one item per query pair, see untiled_splits.
+int diff_splits(int B, int heads, int D, int64_t max_seq, int sm_count) {
+  return untiled_splits(B, heads, heads, D, false, max_seq, sm_count);
+}
+
+int64_t diff_ws_bytes(int B, int heads, int D, int S) {
+  return std::max<int64_t>(static_cast<int64_t>(S) * B * 2 * heads * partial_row_floats(2 * D) * 4, 16);
+}
+
+struct DiffExtra {
+  const void* lam; int lam_dtype; int64_t lam_stride;
+  const void* norm_w; int norm_dtype; float norm_eps; float out_scale;
+};
+
+// `a` in the caller's terms: Hq = query pairs, Hkv = KV pairs, D = head dim.
+int run_diff(const AttnCall& a, const DiffExtra& x) {
+  if (a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.D <= 0 || a.block_size <= 0 || a.num_blocks < 0 || a.bt_width < 0)
+    return INT8KV_E_BAD_SHAPE;
+  if (a.Hq % a.Hkv != 0 || a.num_splits < 0 || a.num_splits > kMaxSplits) return INT8KV_E_BAD_SHAPE;
+  if (!valid_float_dtype(a.q_dtype) || !valid_float_dtype(a.out_dtype) || !valid_float_dtype(x.lam_dtype) ||
+      (x.norm_w != nullptr && !valid_float_dtype(x.norm_dtype)))
+    return INT8KV_E_BAD_DTYPE;
+  if (x.norm_w != nullptr && !(x.norm_eps > 0.f)) return INT8KV_E_BAD_SHAPE;
+  if (a.D > kDiffMaxD) return INT8KV_E_UNSUPPORTED;
+  if (a.B == 0) return INT8KV_OK;
+  if (!a.query || !a.kc || !a.vc || !a.bt || !a.sl || !a.q_st || !a.kc_st || !a.vc_st || !a.bt_st || !a.out || !a.o_st || !x.lam)
+    return INT8KV_E_NULLPTR;
+  if (a.cache_kind == kCacheInt8 && (!a.k_scale || !a.v_scale)) return INT8KV_E_NULLPTR;
+  if (a.kc_st[3] != 1 || a.vc_st[3] != 1) return INT8KV_E_UNSUPPORTED;
+
+  const int sm = device_sm_count();
+  const int64_t cap = a.bt_width * a.block_size;
+  const int64_t max_seq = a.max_seq_hint > 0 ? std::min(a.max_seq_hint, cap) : cap;
+  const int64_t tiles = (max_seq + 15) / 16;
+  int S = a.num_splits > 0 ? a.num_splits : diff_splits(a.B, a.Hq, a.D, max_seq, sm);
+  S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(S, tiles)));
+  if (a.ws == nullptr || a.ws_bytes < diff_ws_bytes(a.B, a.Hq, a.D, S) || (reinterpret_cast<uintptr_t>(a.ws) & 15u))
+    return INT8KV_E_WORKSPACE;
+
+  DiffParams d;
+  std::memset(&d, 0, sizeof(d));
+  d.heads = a.Hq; d.group = a.Hq / a.Hkv; d.Dk = a.D;
+  d.lam = x.lam; d.lam_dtype = x.lam_dtype; d.lam_st = x.lam_stride;
+  d.norm_w = x.norm_w; d.norm_dtype = x.norm_dtype; d.norm_eps = x.norm_eps; d.out_scale = x.out_scale;
+  AttnParams& p = d.a;
+  p.q = a.query; p.q_dtype = a.q_dtype;
+  for (int i = 0; i < 3; ++i) { p.q_st[i] = a.q_st[i]; p.o_st[i] = a.o_st[i]; }
+  p.B = a.B; p.Hq = 2 * a.Hq; p.Hkv = a.Hkv; p.G = 2 * d.group; p.D = 2 * a.D;
+  p.kc = a.kc; p.vc = a.vc; p.cache_kind = a.cache_kind;
+  for (int i = 0; i < 4; ++i) { p.kc_st[i] = a.kc_st[i]; p.vc_st[i] = a.vc_st[i]; }
+  p.num_blocks = a.num_blocks; p.block_size = a.block_size;
+  p.tiles_per_block = a.block_size / 16;
+  p.hint_tiles = static_cast<int>(tiles);
+  p.bt = a.bt; p.bt_is_i64 = a.bt_is_i64; p.bt_st[0] = a.bt_st[0]; p.bt_st[1] = a.bt_st[1]; p.bt_width = a.bt_width;
+  p.sl = a.sl; p.sl_is_i64 = a.sl_is_i64;
+  p.k_scale = a.k_scale; p.v_scale = a.v_scale;
+  p.out = a.out; p.out_dtype = a.out_dtype;
+  p.num_splits = S;
+  p.per_longest = static_cast<int>(std::max<int64_t>(1, (tiles + S - 1) / S));
+  p.row_floats = partial_row_floats(2 * a.D);
+  p.sm_scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(a.D)));
+  p.status = a.status;
+  p.part = reinterpret_cast<float*>(a.ws);
+  const int rc = launch_diff_generic(d, a.stream);
+  return rc != INT8KV_OK ? rc : launch_diff_merge(d, a.stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t int8kv_diff_workspace_bytes(int batch, int num_heads, int num_kv_pairs, int head_dim, int64_t max_seq_len,
+                                    int block_size, int num_splits, int sm_count) {
+  if (batch < 0 || num_heads <= 0 || num_kv_pairs <= 0 || num_heads % num_kv_pairs != 0 || head_dim <= 0 ||
+      max_seq_len < 0 || block_size <= 0 || num_splits < 0 || num_splits > kMaxSplits)
+    return -1;
+  const int sm = sm_count > 0 ? sm_count : 148;
+  const int S = num_splits > 0 ? num_splits : diff_splits(std::max(batch, 1), num_heads, head_dim, max_seq_len, sm);
+  return diff_ws_bytes(batch, num_heads, head_dim, S);
+}
+
+int int8kv_paged_diff_attn_int8(const void* query, int q_dtype, const int64_t q_strides[3], int batch, int num_heads,
+                                int num_kv_pairs, int head_dim, const int8_t* key_cache, const int8_t* value_cache,
+                                const int64_t key_cache_strides[4], const int64_t value_cache_strides[4],
+                                int64_t num_blocks, int block_size, const void* block_tables, int bt_is_i64,
+                                const int64_t bt_strides[2], int64_t bt_width, const void* seq_lens, int sl_is_i64,
+                                int64_t max_seq_len_hint, const float* k_scale, const float* v_scale, const void* lam,
+                                int lam_dtype, int64_t lam_stride, const void* norm_weight, int norm_dtype,
+                                float norm_eps, float out_scale, void* out, int out_dtype, const int64_t out_strides[3],
+                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
+                                void* stream) {
+  AttnCall a{query, q_dtype, q_strides, batch, num_heads, num_kv_pairs, head_dim,
+             key_cache, value_cache, kCacheInt8, key_cache_strides, value_cache_strides, num_blocks, block_size,
+             block_tables, bt_is_i64, bt_strides, bt_width, seq_lens, sl_is_i64, max_seq_len_hint,
+             k_scale, v_scale, out, out_dtype, out_strides, nullptr,
+             num_splits, workspace, workspace_bytes, 0, static_cast<cudaStream_t>(stream)};
+  a.status = status;
+  return run_diff(a, DiffExtra{lam, lam_dtype, lam_stride, norm_weight, norm_dtype, norm_eps, out_scale});
+}
+
+int int8kv_paged_diff_attn_bf16(const void* query, int q_dtype, const int64_t q_strides[3], int batch, int num_heads,
+                                int num_kv_pairs, int head_dim, const void* key_cache, const void* value_cache,
+                                int cache_dtype, const int64_t key_cache_strides[4],
+                                const int64_t value_cache_strides[4], int64_t num_blocks, int block_size,
+                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
+                                const void* seq_lens, int sl_is_i64, int64_t max_seq_len_hint, const void* lam,
+                                int lam_dtype, int64_t lam_stride, const void* norm_weight, int norm_dtype,
+                                float norm_eps, float out_scale, void* out, int out_dtype, const int64_t out_strides[3],
+                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
+                                void* stream) {
+  if (cache_dtype != INT8KV_BF16 && cache_dtype != INT8KV_FP16) return INT8KV_E_BAD_DTYPE;
+  AttnCall a{query, q_dtype, q_strides, batch, num_heads, num_kv_pairs, head_dim,
+             key_cache, value_cache, cache_dtype == INT8KV_BF16 ? kCacheBf16 : kCacheFp16,
+             key_cache_strides, value_cache_strides, num_blocks, block_size,
+             block_tables, bt_is_i64, bt_strides, bt_width, seq_lens, sl_is_i64, max_seq_len_hint,
+             nullptr, nullptr, out, out_dtype, out_strides, nullptr,
+             num_splits, workspace, workspace_bytes, 0, static_cast<cudaStream_t>(stream)};
+  a.status = status;
+  return run_diff(a, DiffExtra{lam, lam_dtype, lam_stride, norm_weight, norm_dtype, norm_eps, out_scale});
+}
+
+}  // extern "C"

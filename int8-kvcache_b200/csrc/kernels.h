@@ -165,6 +165,24 @@ struct ChainedMerge {
   int duty;
 };
 
+// Differential attention (paged_diff_attn.cu).  `a` describes the call in terms of partial rows: a.Hq = 2 * heads rows per
+// sequence (row 2h + map), a.Hkv = KV pairs, a.G = 2 * group, a.D = 2 * Dk values per row; its query and cache strides
+// are those of the tensors, [B, 2 * heads, Dk] and [num_blocks, BS, 2 * pairs, Dk].
+struct DiffParams {
+  AttnParams a;
+  int heads, group, Dk;
+  const void* lam;     // [heads], stride lam_st (0: one value for all heads)
+  int lam_dtype;
+  int64_t lam_st;
+  const void* norm_w;  // [2 * Dk] or null: no norm
+  int norm_dtype;
+  float norm_eps;
+  float out_scale;
+};
+constexpr int kDiffMaxD = 256;
+int launch_diff_generic(const DiffParams& d, cudaStream_t stream);
+int launch_diff_merge(const DiffParams& d, cudaStream_t stream);
+
 // Block tables and slot maps (block_tables.cu).
 // What the write phase needs of a request.
 struct alignas(16) TabRecord {

@@ -1,0 +1,67 @@
+"""Differential attention without a GPU: the checker against the elementary formula, refusals of host tensors, and the
+argument checks of the C ABI."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from conftest import package
+from oracle.diff_attention import diff_paged_attention
+
+
+def test_checker_is_the_difference_of_two_ordinary_attentions():
+    """Against the fp32 checker of ordinary decode attention, run once per map and half of V."""
+    import oracle
+
+    torch.manual_seed(0)
+    B, H, P, D, bs = 2, 6, 2, 16, 16
+    q = torch.randn(B, 2 * H, D)
+    kc, vc = torch.randn(5, bs, 2 * P, D, dtype=torch.float64).to(torch.bfloat16), torch.randn(5, bs, 2 * P, D).to(torch.bfloat16)
+    bt = torch.tensor([[3, 1, 0], [4, 2, 0]])
+    lens, lam = [40, 7], torch.rand(H)
+    want, _ = diff_paged_attention(q, kc, vc, bt, lens, lam)
+    pick = lambda c, m: c[:, :, m::2].contiguous()
+    for half in range(2):
+        maps = [oracle.float_paged_attention_oracle(q[:, m::2].contiguous(), pick(kc, m), pick(vc, half), bt, lens) for m in range(2)]
+        got = maps[0] - lam[None, :, None] * maps[1]
+        assert (got - want[..., half * D:(half + 1) * D]).abs().max() < 1e-5
+
+
+def test_entry_points_refuse_host_tensors(kv):
+    q, c = torch.zeros(1, 4, 64), torch.zeros(1, 16, 2, 64, dtype=torch.int8)
+    args = (torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32))
+    with pytest.raises(AssertionError):
+        kv.int8_paged_diff_attention(q, c, c, *args, torch.ones(2), torch.ones(2), torch.ones(2))
+    with pytest.raises(AssertionError):
+        kv.bf16_paged_diff_attention(q, c.bfloat16(), c.bfloat16(), *args, torch.ones(2))
+
+
+def test_c_abi_argument_checks():
+    lm = package("_lib")
+    lib = lm.load()
+    p = C.c_void_p(256)  # never dereferenced: every call below is refused
+    s3, s4, s2 = lm.i64((512, 128, 1)), lm.i64((8192, 512, 128, 1)), lm.i64((4, 1))
+
+    def call(B=2, H=4, P=2, D=128, bs=16, q=p, lam=p, ks=p, qd=lm.BF16, ld=lm.FP32, norm=None, eps=1e-5, splits=1, ws=p,
+             ws_bytes=1 << 20, st=s4, out=p):
+        return lib.int8kv_paged_diff_attn_int8(q, qd, s3, B, H, P, D, p, p, st, st, 4, bs, p, 0, s2, 4, p, 0, 64, ks, p,
+                                               lam, ld, 1, norm, lm.FP32, eps, 1.0, out, lm.BF16, s3, splits, ws, ws_bytes,
+                                               None, None)
+
+    assert call(B=0) == lm.OK
+    assert call(B=-1) == lm.E_BAD_SHAPE and call(H=3) == lm.E_BAD_SHAPE and call(P=0) == lm.E_BAD_SHAPE
+    assert call(bs=0) == lm.E_BAD_SHAPE and call(splits=-1) == lm.E_BAD_SHAPE and call(splits=1000) == lm.E_BAD_SHAPE
+    assert call(qd=7) == lm.E_BAD_DTYPE and call(ld=-1) == lm.E_BAD_DTYPE
+    assert call(norm=p, eps=0.0) == lm.E_BAD_SHAPE and call(norm=p, eps=float("nan")) == lm.E_BAD_SHAPE
+    assert call(D=257) == lm.E_UNSUPPORTED and call(st=lm.i64((8192, 512, 128, 2))) == lm.E_UNSUPPORTED
+    for missing in ("q", "lam", "ks", "out"):
+        assert call(**{missing: None}) == lm.E_NULLPTR
+    need = lib.int8kv_diff_workspace_bytes(2, 4, 2, 128, 64, 16, 1, 148)
+    assert need == 2 * 8 * 260 * 4
+    assert call(ws=None) == lm.E_WORKSPACE and call(ws_bytes=need - 1) == lm.E_WORKSPACE
+    assert call(ws=C.c_void_p(264)) == lm.E_WORKSPACE
+    assert lib.int8kv_diff_workspace_bytes(2, 3, 2, 128, 64, 16, 1, 148) == -1
+    assert lib.int8kv_paged_diff_attn_bf16(p, lm.BF16, s3, 2, 4, 2, 128, p, p, lm.FP32, s4, s4, 4, 16, p, 0, s2, 4, p, 0,
+                                           64, p, lm.FP32, 1, None, 0, 1e-5, 1.0, p, lm.BF16, s3, 1, p, 1 << 20, None,
+                                           None) == lm.E_BAD_DTYPE
