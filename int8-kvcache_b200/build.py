@@ -19,7 +19,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libint8kv_b200.so"
 SOURCES = ["c_api.cu", "cache_write.cu", "paged_attn.cu", "block_tables.cu", "paged_diff_attn.cu"]
-HEADERS = ["common.cuh", "kernels.h", "../../include/int8kv_b200.h"]
+HEADERS = ["common.cuh", "paged_items.cuh", "kernels.h", "../../include/int8kv_b200.h"]
 
 NVCC_FLAGS = [
     "-gencode",

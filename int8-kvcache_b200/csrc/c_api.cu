@@ -45,16 +45,16 @@ EncodeTiledFn encode_tiled_fn() {
 }
 
 // Tensor map over a cache [num_blocks, BS, Hkv, row_bytes] viewed in bytes as
-// (byte-in-row, token-in-block, head, block) with a 128 B x 16 token box and the 128-byte swizzle.
+// (byte-in-row, token-in-block, head, block) with a 128 B x 16 token x heads_per_box box and the 128-byte swizzle.
 bool make_cache_map(CUtensorMap* map, const void* base, int elem_bytes, int D, int Hkv, int64_t num_blocks,
-                    int block_size, const int64_t st[4]) {
+                    int block_size, const int64_t st[4], int heads_per_box = 1) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (enc == nullptr) return false;
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D) * elem_bytes, static_cast<cuuint64_t>(block_size),
                               static_cast<cuuint64_t>(Hkv), static_cast<cuuint64_t>(num_blocks)};
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(st[1]) * elem_bytes, static_cast<cuuint64_t>(st[2]) * elem_bytes,
                                  static_cast<cuuint64_t>(st[0]) * elem_bytes};
-  const cuuint32_t box[4] = {128, 16, 1, 1};
+  const cuuint32_t box[4] = {128, 16, static_cast<cuuint32_t>(heads_per_box), 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -92,7 +92,8 @@ static int64_t pow2_floor(int64_t x) {
 // latency-driven count is capped at 16 parts (measured on the 8 x 4096-token cell, per layer: 32 parts 11.1 us, of
 // which the second round trip of the merge is about 2 us) and the rule that cuts the smallest calls into more,
 // shorter parts is left out.
-int choose_splits(int B, int Hkv, int64_t max_seq, int block_size, int sm_count, bool chained = false) {
+int choose_splits(int B, int Hkv, int64_t max_seq, int block_size, int sm_count, bool chained = false,
+                  int warps_per_sm = 12) {
   (void)block_size;
   if (B <= 0 || Hkv <= 0 || max_seq <= 0) return 1;
   const int64_t tiles = (max_seq + 15) / 16;
@@ -103,7 +104,7 @@ int choose_splits(int B, int Hkv, int64_t max_seq, int block_size, int sm_count,
   //    warps, down to 2 tiles per part for short sequences (16 parts) and 8 tiles per part for long ones;
   //  * large calls are bound by HBM, where ragged batches balance best with about four waves of warps, but a part
   //    of fewer than 32 tiles would spend too much of its traffic on its partial rows.
-  const int64_t slots = static_cast<int64_t>(sm_count) * 12;
+  const int64_t slots = static_cast<int64_t>(sm_count) * warps_per_sm;
   const int64_t by_latency = chained ? std::min<int64_t>(tiles / 2, 16)
                                      : std::min<int64_t>(tiles / 2, std::max<int64_t>(16, tiles / 8));
   int64_t s_fill = std::min(pow2_floor(std::max<int64_t>(1, slots / items)), pow2_floor(std::max<int64_t>(1, by_latency)));
@@ -156,22 +157,22 @@ int env_int_or(const char* name, int fallback) {
 // Whether the shape can be planned at all: every warp walks seq_lens a few times, which stays cheap up to a few
 // hundred sequences, and one part per (sequence, head) must fit one wave.
 constexpr int kPlanMaxBatch = 512;
-bool plan_possible(int B, int Hkv, int sm_count) {
-  return B <= kPlanMaxBatch && static_cast<int64_t>(B) * Hkv <= static_cast<int64_t>(sm_count) * 12;
+bool plan_possible(int B, int Hkv, int sm_count, int warps_per_sm = 12) {
+  return B <= kPlanMaxBatch && static_cast<int64_t>(B) * Hkv <= static_cast<int64_t>(sm_count) * warps_per_sm;
 }
 
 // Whether planning pays: enough nominal work for one wave of parts of at least 12 tiles, and a split
 // heuristic that could not reach four waves of warps for this shape (with four or more waves the tail is small and
 // the plan's longer prologue, every warp reading seq_lens before its block table, costs more than it gains:
 // measured 222 us against 216 us per call on the 256-sequence ragged batch).
-bool plan_pays(int B, int Hkv, int64_t max_seq, int block_size, int sm_count) {
+bool plan_pays(int B, int Hkv, int64_t max_seq, int block_size, int sm_count, int warps_per_sm = 12) {
   static const int enabled = env_int_or("INT8KV_PLAN", 1);
-  if (!enabled || !plan_possible(B, Hkv, sm_count)) return false;
-  const int64_t slots = static_cast<int64_t>(sm_count) * 12;
+  if (!enabled || !plan_possible(B, Hkv, sm_count, warps_per_sm)) return false;
+  const int64_t slots = static_cast<int64_t>(sm_count) * warps_per_sm;
   const int64_t items = static_cast<int64_t>(B) * Hkv;
   const int64_t tiles = (max_seq + 15) / 16;
   if (items * tiles < slots * 12) return false;
-  return items * choose_splits(B, Hkv, max_seq, block_size, sm_count) < slots * 4;
+  return items * choose_splits(B, Hkv, max_seq, block_size, sm_count, false, warps_per_sm) < slots * 4;
 }
 
 // Warps per SM that a plan counts as one wave.  A single call fills the machine exactly (12 resident warps per SM).
@@ -1088,13 +1089,43 @@ int int8kv_release_block_tables(const void* seq_lens, int sl_is_i64, const uint8
 // =============================================================================================================
 namespace {
 
-// Split count of the kernel for every shape: one item per query pair, see untiled_splits.
-int diff_splits(int B, int heads, int D, int64_t max_seq, int sm_count) {
-  return untiled_splits(B, heads, heads, D, false, max_seq, sm_count);
+// How a call is cut, decided from its shape alone.
+struct DiffPlan {
+  bool planned;      // parts planned on the device from the lengths
+  int S;             // parts per sequence otherwise
+  PlanShape ps;
+  int64_t table_off; // planned: offset of the sequence table behind the partial rows
+  int64_t need;      // workspace bytes
+};
+
+int64_t diff_rows_bytes(int64_t rows, int D) { return rows * partial_row_floats(2 * D) * 4; }
+
+// tiled: the TMA-tiled kernels serve the shape; they split as the ordinary tiled ones do, on the warps that an SM holds of
+// them.  Otherwise one item per query pair, see untiled_splits.
+DiffPlan diff_plan(bool tiled, int cache_kind, int B, int heads, int pairs, int D, int64_t max_seq, int64_t cap, int block_size,
+                   int num_splits, int sm) {
+  DiffPlan t;
+  std::memset(&t, 0, sizeof(t));
+  const int64_t tiles = (max_seq + 15) / 16;
+  const int wps = diff_warps_per_sm(cache_kind, D, heads / pairs);
+  t.planned = tiled && num_splits == 0 && tiles > 0 && cap < (int64_t(1) << 21) * 16 &&
+              plan_pays(B, pairs, max_seq, block_size, sm, wps);
+  if (t.planned) {
+    t.ps = plan_shape(B, pairs, tiles, sm, wps);
+    t.S = kMaxSplits;  // upper bound of the parts of one sequence
+    t.table_off = diff_rows_bytes(static_cast<int64_t>(t.ps.max_items) * 2 * (heads / pairs), D);
+    t.need = t.table_off + static_cast<int64_t>(B) * 8;
+    return t;
+  }
+  int64_t S = num_splits;
+  if (S == 0) S = tiled ? choose_splits(B, pairs, max_seq, block_size, sm, false, wps) : untiled_splits(B, heads, heads, D, false, max_seq, sm);
+  t.S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(S, tiles)));
+  t.need = std::max<int64_t>(diff_rows_bytes(static_cast<int64_t>(t.S) * B * 2 * heads, D), 16);
+  return t;
 }
 
-int64_t diff_ws_bytes(int B, int heads, int D, int S) {
-  return std::max<int64_t>(static_cast<int64_t>(S) * B * 2 * heads * partial_row_floats(2 * D) * 4, 16);
+bool diff_tiled_shape(int D, int group, int block_size) {
+  return (D == 64 || D == 128) && group <= 8 && block_size % 16 == 0;
 }
 
 struct DiffExtra {
@@ -1122,10 +1153,14 @@ int run_diff(const AttnCall& a, const DiffExtra& x) {
   const int64_t cap = a.bt_width * a.block_size;
   const int64_t max_seq = a.max_seq_hint > 0 ? std::min(a.max_seq_hint, cap) : cap;
   const int64_t tiles = (max_seq + 15) / 16;
-  int S = a.num_splits > 0 ? a.num_splits : diff_splits(a.B, a.Hq, a.D, max_seq, sm);
-  S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(S, tiles)));
-  if (a.ws == nullptr || a.ws_bytes < diff_ws_bytes(a.B, a.Hq, a.D, S) || (reinterpret_cast<uintptr_t>(a.ws) & 15u))
-    return INT8KV_E_WORKSPACE;
+  const bool int8_cache = a.cache_kind == kCacheInt8;
+  const int esz = int8_cache ? 1 : 2;
+  // INT8 rows of 64 values: the two heads of a pair are staged as one row, so they have to be neighbours
+  const bool pair_rows = int8_cache && a.D == 64;
+  const bool tiled = diff_tiled_shape(a.D, a.Hq / a.Hkv, a.block_size) && tma_friendly(a.kc, esz, a.kc_st, a.num_blocks) &&
+                     tma_friendly(a.vc, esz, a.vc_st, a.num_blocks) && (!pair_rows || (a.kc_st[2] == 64 && a.vc_st[2] == 64));
+  const DiffPlan t = diff_plan(tiled, a.cache_kind, a.B, a.Hq, a.Hkv, a.D, max_seq, cap, a.block_size, a.num_splits, sm);
+  if (a.ws == nullptr || a.ws_bytes < t.need || (reinterpret_cast<uintptr_t>(a.ws) & 15u)) return INT8KV_E_WORKSPACE;
 
   DiffParams d;
   std::memset(&d, 0, sizeof(d));
@@ -1145,14 +1180,34 @@ int run_diff(const AttnCall& a, const DiffExtra& x) {
   p.sl = a.sl; p.sl_is_i64 = a.sl_is_i64;
   p.k_scale = a.k_scale; p.v_scale = a.v_scale;
   p.out = a.out; p.out_dtype = a.out_dtype;
-  p.num_splits = S;
-  p.per_longest = static_cast<int>(std::max<int64_t>(1, (tiles + S - 1) / S));
+  p.num_splits = t.S;
+  p.per_longest = static_cast<int>(std::max<int64_t>(1, (tiles + t.S - 1) / t.S));
   p.row_floats = partial_row_floats(2 * a.D);
   p.sm_scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(a.D)));
   p.status = a.status;
   p.part = reinterpret_cast<float*>(a.ws);
-  const int rc = launch_diff_generic(d, a.stream);
-  return rc != INT8KV_OK ? rc : launch_diff_merge(d, a.stream);
+  if (!tiled) {
+    const int rc = launch_diff_generic(d, a.stream);
+    return rc != INT8KV_OK ? rc : launch_diff_merge(d, a.stream);
+  }
+  if (t.planned) {
+    p.plan_table = reinterpret_cast<int2*>(static_cast<char*>(a.ws) + t.table_off);
+    p.plan_grid_items = t.ps.max_items;
+    p.plan_slots = sm * diff_warps_per_sm(a.cache_kind, a.D, d.group);
+    p.plan_k_max = t.ps.k_max;
+    p.plan_min_part = t.ps.min_part;
+  } else if (t.S == 1) {
+    p.part = nullptr;  // whole sequences: the attention kernel writes `out`
+  }
+  alignas(64) CUtensorMap tmK, tmV;
+  auto map = [&](CUtensorMap* m, const void* base, const int64_t* st) {
+    const int64_t pair_st[4] = {st[0], st[1], 2 * st[2], 1};
+    return pair_rows ? make_cache_map(m, base, 1, 128, a.Hkv, a.num_blocks, a.block_size, pair_st)
+                     : make_cache_map(m, base, esz, a.D, 2 * a.Hkv, a.num_blocks, a.block_size, st, 2);
+  };
+  if (!map(&tmK, a.kc, a.kc_st) || !map(&tmV, a.vc, a.vc_st)) return INT8KV_E_LAUNCH;
+  const int rc = launch_diff_tiled(d, tmK, tmV, sm, a.stream);
+  return rc != INT8KV_OK || t.S == 1 ? rc : launch_diff_merge(d, a.stream);
 }
 
 }  // namespace
@@ -1165,8 +1220,17 @@ int64_t int8kv_diff_workspace_bytes(int batch, int num_heads, int num_kv_pairs, 
       max_seq_len < 0 || block_size <= 0 || num_splits < 0 || num_splits > kMaxSplits)
     return -1;
   const int sm = sm_count > 0 ? sm_count : 148;
-  const int S = num_splits > 0 ? num_splits : diff_splits(std::max(batch, 1), num_heads, head_dim, max_seq_len, sm);
-  return diff_ws_bytes(batch, num_heads, head_dim, S);
+  int64_t need = 16;
+  for (const int kind : {static_cast<int>(kCacheInt8), static_cast<int>(kCacheBf16)})
+    for (const bool tiled : {true, false}) {  // alignment and strides, which are not known here, decide between the two
+      if (tiled && !diff_tiled_shape(head_dim, num_heads / num_kv_pairs, block_size)) continue;
+      need = std::max(need, diff_plan(tiled, kind, batch, num_heads, num_kv_pairs, head_dim, max_seq_len, max_seq_len,
+                                      block_size, num_splits, sm).need);
+      // a table too wide for a device plan falls back to the fixed count
+      need = std::max(need, diff_plan(tiled, kind, batch, num_heads, num_kv_pairs, head_dim, max_seq_len,
+                                      int64_t(1) << 40, block_size, num_splits, sm).need);
+    }
+  return need;
 }
 
 int int8kv_paged_diff_attn_int8(const void* query, int q_dtype, const int64_t q_strides[3], int batch, int num_heads,
