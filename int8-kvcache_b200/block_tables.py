@@ -14,15 +14,15 @@ captured in a CUDA graph.  The reference builds both on the host (tests/test_int
 
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
-from .ops import _require_lib, _stream_ptr
+from .ops import _call, _require_lib
 
-_INDEX = (torch.int32, torch.int64)
+_INDEX_CODES = {torch.int32: 0, torch.int64: 1}
+_MAX_TOKENS = 2**31 - 1
 
 
 class BlockTableStep(NamedTuple):
@@ -34,29 +34,25 @@ class BlockTableStep(NamedTuple):
     free_cursor: torch.Tensor  # [1] int64
 
 
-def _on_device(device: torch.device):
-    """The launch context of `device`: a no-op when it is the current one already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _check_lists(device, block_tables, seq_lens, block_size, written):
-    assert block_tables.is_cuda and block_tables.ndim == 2 and block_tables.dtype in _INDEX
-    assert seq_lens.ndim == 1 and seq_lens.dtype in _INDEX and seq_lens.device == device
-    assert seq_lens.numel() == block_tables.shape[0]
-    assert int(block_size) > 0
-    if written:  # an expanded table has one memory cell for several entries
-        assert all(st != 0 or n <= 1 for st, n in zip(block_tables.stride(), block_tables.shape))
+def _check_lists(block_tables, seq_lens, block_size):
+    """(device, requests, width, index code of the table, of the lengths)"""
+    device = block_tables.device
+    assert device.type == "cuda" and block_tables.ndim == 2 and seq_lens.ndim == 1 and seq_lens.device == device
+    requests, width = block_tables.shape
+    bt_code, sl_code = _INDEX_CODES.get(block_tables.dtype), _INDEX_CODES.get(seq_lens.dtype)
+    assert bt_code is not None and sl_code is not None and seq_lens.shape[0] == requests and block_size > 0
+    return device, requests, width, bt_code, sl_code
 
 
 def _check_free_list(device, free_blocks, free_cursor):
-    assert free_blocks.ndim == 1 and free_blocks.dtype in _INDEX and free_blocks.device == device
+    code = _INDEX_CODES.get(free_blocks.dtype)
+    assert free_blocks.ndim == 1 and code is not None and free_blocks.device == device
     assert free_cursor.numel() == 1 and free_cursor.dtype == torch.int64 and free_cursor.device == device
+    return code
 
 
-def _check_out(out, like, shape, dtype):
-    assert out.shape == shape and out.dtype == dtype and out.device == like.device and out.is_contiguous()
+def _check_out(out, device, shape, dtype):
+    assert out.shape == shape and out.dtype == dtype and out.device == device and out.is_contiguous()
 
 
 def _workspace(lib, requests: int, items: int, device) -> Tuple[Optional[torch.Tensor], int, int]:
@@ -88,37 +84,34 @@ def build_block_tables(
     blocks when the list has not enough left, is refused: no blocks, the old length, slots -1.
     out: preallocated outputs; its seq_lens and free_cursor may be the inputs themselves, which then advance in place.
     """
-    device = block_tables.device
-    _check_lists(device, block_tables, seq_lens, block_size, True)
-    _check_free_list(device, free_blocks, free_cursor)
-    R, width = block_tables.shape
-    num_tokens = int(num_tokens)
-    assert new_lens.ndim == 1 and new_lens.numel() == R and new_lens.dtype in _INDEX and new_lens.device == device
-    assert 0 <= num_tokens < 2**31 - 1
+    device, R, width, bt_code, sl_code = _check_lists(block_tables, seq_lens, block_size)
+    bt_st = block_tables.stride()  # an expanded table has one memory cell for several entries
+    assert (bt_st[0] != 0 or R <= 1) and (bt_st[1] != 0 or width <= 1)
+    fb_code, nl_code = _check_free_list(device, free_blocks, free_cursor), _INDEX_CODES.get(new_lens.dtype)
+    assert new_lens.shape == seq_lens.shape and nl_code is not None and new_lens.device == device
+    assert 0 <= num_tokens < _MAX_TOKENS
     if out is None:
         out = BlockTableStep(torch.empty(num_tokens, dtype=torch.int64, device=device),
                              torch.empty(R + 1, dtype=torch.int32, device=device),
-                             torch.empty(R, dtype=seq_lens.dtype, device=device),
-                             torch.empty(1, dtype=torch.int64, device=device))
+                             seq_lens.new_empty(R), free_cursor.new_empty(1))
     else:
-        _check_out(out.slot_mapping, block_tables, (num_tokens,), torch.int64)
-        _check_out(out.query_start, block_tables, (R + 1,), torch.int32)
-        _check_out(out.seq_lens, block_tables, (R,), seq_lens.dtype)
-        _check_out(out.free_cursor, block_tables, (1,), torch.int64)
+        _check_out(out.slot_mapping, device, (num_tokens,), torch.int64)
+        _check_out(out.query_start, device, (R + 1,), torch.int32)
+        _check_out(out.seq_lens, device, (R,), seq_lens.dtype)
+        _check_out(out.free_cursor, device, (1,), torch.int64)
     lib = _require_lib()
     seq_lens, new_lens, free_blocks = seq_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
-    ws, ws_ptr, ws_bytes = _workspace(lib, R, num_tokens + num_tokens // int(block_size) + R, device)
-    with _on_device(device):
-        rc = lib.int8kv_build_block_tables(
-            seq_lens.data_ptr(), int(seq_lens.dtype == torch.int64),
-            new_lens.data_ptr(), int(new_lens.dtype == torch.int64), R, int(block_size),
-            block_tables.data_ptr(), int(block_tables.dtype == torch.int64), _lib.i64(block_tables.stride()), width,
-            free_blocks.data_ptr(), int(free_blocks.dtype == torch.int64), free_blocks.numel(),
-            free_cursor.data_ptr(), out.free_cursor.data_ptr(), out.seq_lens.data_ptr(),
-            out.slot_mapping.data_ptr(), num_tokens, out.query_start.data_ptr(),
-            ws_ptr, ws_bytes, _stream_ptr(device),
-        )
-    _lib.check("int8kv_build_block_tables", rc)
+    ws, ws_ptr, ws_bytes = _workspace(lib, R, num_tokens + num_tokens // block_size + R, device)
+    rc = _call(
+        device, lib.int8kv_build_block_tables,
+        seq_lens.data_ptr(), sl_code, new_lens.data_ptr(), nl_code, R, block_size,
+        block_tables.data_ptr(), bt_code, _lib.i64(bt_st), width,
+        free_blocks.data_ptr(), fb_code, free_blocks.shape[0],
+        free_cursor.data_ptr(), out.free_cursor.data_ptr(), out.seq_lens.data_ptr(),
+        out.slot_mapping.data_ptr(), num_tokens, out.query_start.data_ptr(), ws_ptr, ws_bytes,
+    )
+    if rc != _lib.OK:
+        _lib.check("int8kv_build_block_tables", rc)
     return out
 
 
@@ -134,29 +127,27 @@ def build_slot_mapping(
     """(slot_mapping [num_tokens] int64, query_start [R + 1] int32) of new_lens[b] tokens that follow the seq_lens[b]
     cached ones of request b, through tables that hold their blocks already.  Packing and padding as in
     build_block_tables; a token beyond its table row, or on a negative block id, gets slot -1."""
-    device = block_tables.device
-    _check_lists(device, block_tables, seq_lens, block_size, False)
-    R, width = block_tables.shape
-    num_tokens = int(num_tokens)
-    assert new_lens.ndim == 1 and new_lens.numel() == R and new_lens.dtype in _INDEX and new_lens.device == device
-    assert 0 <= num_tokens < 2**31 - 1
+    device, R, width, bt_code, sl_code = _check_lists(block_tables, seq_lens, block_size)
+    nl_code = _INDEX_CODES.get(new_lens.dtype)
+    assert new_lens.shape == seq_lens.shape and nl_code is not None and new_lens.device == device
+    assert 0 <= num_tokens < _MAX_TOKENS
     if out is None:
         out = (torch.empty(num_tokens, dtype=torch.int64, device=device),
                torch.empty(R + 1, dtype=torch.int32, device=device))
     else:
-        _check_out(out[0], block_tables, (num_tokens,), torch.int64)
-        _check_out(out[1], block_tables, (R + 1,), torch.int32)
+        _check_out(out[0], device, (num_tokens,), torch.int64)
+        _check_out(out[1], device, (R + 1,), torch.int32)
     lib = _require_lib()
     seq_lens, new_lens = seq_lens.contiguous(), new_lens.contiguous()
     ws, ws_ptr, ws_bytes = _workspace(lib, R, num_tokens, device)
-    with _on_device(device):
-        rc = lib.int8kv_build_slot_mapping(
-            seq_lens.data_ptr(), int(seq_lens.dtype == torch.int64),
-            new_lens.data_ptr(), int(new_lens.dtype == torch.int64), R, int(block_size),
-            block_tables.data_ptr(), int(block_tables.dtype == torch.int64), _lib.i64(block_tables.stride()), width,
-            out[0].data_ptr(), num_tokens, out[1].data_ptr(), ws_ptr, ws_bytes, _stream_ptr(device),
-        )
-    _lib.check("int8kv_build_slot_mapping", rc)
+    rc = _call(
+        device, lib.int8kv_build_slot_mapping,
+        seq_lens.data_ptr(), sl_code, new_lens.data_ptr(), nl_code, R, block_size,
+        block_tables.data_ptr(), bt_code, _lib.i64(block_tables.stride()), width,
+        out[0].data_ptr(), num_tokens, out[1].data_ptr(), ws_ptr, ws_bytes,
+    )
+    if rc != _lib.OK:
+        _lib.check("int8kv_build_slot_mapping", rc)
     return out
 
 
@@ -174,26 +165,26 @@ def release_block_tables(
     just below the cursor, in request order.  Returns (seq_lens with 0 for the finished ones, free_cursor); out:
     preallocated outputs, which may be the inputs themselves.  The table is not written.  Every block of a list is
     handed out once, so requests that share blocks must not both be released."""
-    device = block_tables.device
-    _check_lists(device, block_tables, seq_lens, block_size, False)
-    _check_free_list(device, free_blocks, free_cursor)
-    R, width = block_tables.shape
-    assert finished.ndim == 1 and finished.numel() == R and finished.dtype == torch.bool and finished.device == device
+    device, R, width, bt_code, sl_code = _check_lists(block_tables, seq_lens, block_size)
+    fb_code = _check_free_list(device, free_blocks, free_cursor)
+    assert finished.shape == seq_lens.shape and finished.dtype == torch.bool and finished.device == device
     assert free_blocks.is_contiguous()
     if out is None:
-        out = (torch.empty(R, dtype=seq_lens.dtype, device=device), torch.empty(1, dtype=torch.int64, device=device))
+        out = (seq_lens.new_empty(R), free_cursor.new_empty(1))
     else:
-        _check_out(out[0], block_tables, (R,), seq_lens.dtype)
-        _check_out(out[1], block_tables, (1,), torch.int64)
+        _check_out(out[0], device, (R,), seq_lens.dtype)
+        _check_out(out[1], device, (1,), torch.int64)
     lib = _require_lib()
     seq_lens, finished = seq_lens.contiguous(), finished.contiguous()
-    ws, ws_ptr, ws_bytes = _workspace(lib, R, min(R * width, free_blocks.numel()), device)
-    with _on_device(device):
-        rc = lib.int8kv_release_block_tables(
-            seq_lens.data_ptr(), int(seq_lens.dtype == torch.int64), finished.data_ptr(), R, int(block_size),
-            block_tables.data_ptr(), int(block_tables.dtype == torch.int64), _lib.i64(block_tables.stride()), width,
-            free_blocks.data_ptr(), int(free_blocks.dtype == torch.int64), free_blocks.numel(),
-            free_cursor.data_ptr(), out[1].data_ptr(), out[0].data_ptr(), ws_ptr, ws_bytes, _stream_ptr(device),
-        )
-    _lib.check("int8kv_release_block_tables", rc)
+    N = free_blocks.shape[0]
+    ws, ws_ptr, ws_bytes = _workspace(lib, R, min(R * width, N), device)
+    rc = _call(
+        device, lib.int8kv_release_block_tables,
+        seq_lens.data_ptr(), sl_code, finished.data_ptr(), R, block_size,
+        block_tables.data_ptr(), bt_code, _lib.i64(block_tables.stride()), width,
+        free_blocks.data_ptr(), fb_code, N,
+        free_cursor.data_ptr(), out[1].data_ptr(), out[0].data_ptr(), ws_ptr, ws_bytes,
+    )
+    if rc != _lib.OK:
+        _lib.check("int8kv_release_block_tables", rc)
     return out

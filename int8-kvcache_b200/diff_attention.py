@@ -16,65 +16,80 @@ Argument violations raise AssertionError, as in the other operators.  The refere
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .block_tables import _on_device
-from .ops import (_FLOAT_CODES, _as_f32_scale, _check_decode_args, _max_seq_len, _require_lib, _sm_count, _stream_ptr,
-                  _workspace)
+from .ops import _FLOAT_CODES, _as_f32_scale, _call, _max_seq_len, _require_lib, _sm_count, _status_ptr
+
+_INDEX_CODES = {torch.int32: 0, torch.int64: 1}
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(B, H, P, D, max_seq, block_size, splits, sm_count) -> int:
+    return _require_lib().int8kv_diff_workspace_bytes(B, H, P, D, max_seq, block_size, splits, sm_count)
 
 
 def _run(int8, query, key_cache, value_cache, block_tables, seq_lens, k_scale, v_scale, lam, norm_weight, norm_eps,
          out_scale, num_splits, max_seq_len, out):
-    B, Hq, Hkv, D, block_size = _check_decode_args(query, key_cache, value_cache, block_tables, seq_lens)
     device = query.device
-    assert Hq % 2 == 0 and Hkv % 2 == 0 and D <= 256
-    H, P = Hq // 2, Hkv // 2
+    assert device.type == "cuda" and query.ndim == 3 and key_cache.ndim == 4
     for t in (key_cache, value_cache, block_tables, seq_lens, lam):
         assert t.device == device
-    assert lam.dtype in _FLOAT_CODES and lam.ndim <= 1 and lam.numel() in (1, H)
+    B, Hq, D = query.shape
+    num_blocks, block_size, Hkv, cache_D = key_cache.shape
+    kc_st, vc_st, bt_st = key_cache.stride(), value_cache.stride(), block_tables.stride()
+    assert value_cache.shape == key_cache.shape and cache_D == D and kc_st[3] == 1 and vc_st[3] == 1
+    assert Hq % 2 == 0 and Hkv % 2 == 0 and Hkv > 0 and Hq % Hkv == 0 and 0 < D <= 256
+    assert block_tables.ndim == 2 and block_tables.shape[0] == B and seq_lens.ndim == 1 and seq_lens.shape[0] == B
+    q_code, lam_code = _FLOAT_CODES.get(query.dtype), _FLOAT_CODES.get(lam.dtype)
+    bt_code, sl_code = _INDEX_CODES.get(block_tables.dtype), _INDEX_CODES.get(seq_lens.dtype)
+    assert None not in (q_code, lam_code, bt_code, sl_code)
+    H, P = Hq // 2, Hkv // 2
+    lams = lam.numel()
+    assert lam.ndim <= 1 and (lams == 1 or lams == H)
+    norm_ptr = norm_code = 0
     if norm_weight is not None:
-        assert norm_weight.dtype in _FLOAT_CODES and norm_weight.shape == (2 * D,) and norm_weight.device == device
-        assert norm_eps > 0
+        norm_code = _FLOAT_CODES.get(norm_weight.dtype)
+        assert norm_code is not None and norm_weight.shape == (2 * D,) and norm_weight.device == device and norm_eps > 0
         norm_weight = norm_weight.contiguous()
-    assert num_splits is None or int(num_splits) >= 1
-    max_seq = _max_seq_len(seq_lens, block_tables, block_size, max_seq_len)
+        norm_ptr = norm_weight.data_ptr()
     if out is None:
-        out = torch.empty((B, H, 2 * D), device=device, dtype=query.dtype)
+        out, out_code = query.new_empty((B, H, 2 * D)), q_code
     else:
-        assert out.shape == (B, H, 2 * D) and out.dtype in _FLOAT_CODES and out.device == device
+        out_code = _FLOAT_CODES.get(out.dtype)
+        assert out.shape == (B, H, 2 * D) and out_code is not None and out.device == device
+    splits = 0
+    lib = _require_lib()
+    if num_splits is not None:
+        assert int(num_splits) >= 1
+        splits = min(int(num_splits), lib.int8kv_max_splits())
+    max_seq = _max_seq_len(seq_lens, block_tables, block_size, max_seq_len)
     if B == 0:
         return out
     if seq_lens.stride(0) != 1:
         seq_lens = seq_lens.contiguous()
-    lib = _require_lib()
-    splits = 0 if num_splits is None else min(int(num_splits), lib.int8kv_max_splits())
-    limit = block_tables.shape[1] * block_size
-    nbytes = lib.int8kv_diff_workspace_bytes(B, H, P, D, min(max_seq, limit) if max_seq > 0 else limit, block_size,
-                                             splits, _sm_count(device))
-    with _on_device(device):
-        # The partial rows belong to the call: memory of the current stream, or of the pool of the graph that captures
-        # the call.  The status word is the stream's, the one that device_status() reads.
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        shared = _workspace(device, 16)
-        status = shared.data_ptr() + lib.int8kv_workspace_status_offset(shared.numel())
-        head = (query.data_ptr(), _FLOAT_CODES[query.dtype], _lib.i64(query.stride()), B, H, P, D,
-                key_cache.data_ptr(), value_cache.data_ptr())
-        mid = (_lib.i64(key_cache.stride()), _lib.i64(value_cache.stride()), key_cache.shape[0], block_size,
-               block_tables.data_ptr(), int(block_tables.dtype == torch.int64), _lib.i64(block_tables.stride()),
-               block_tables.shape[1], seq_lens.data_ptr(), int(seq_lens.dtype == torch.int64), max_seq)
-        tail = (lam.data_ptr(), _FLOAT_CODES[lam.dtype], 0 if lam.numel() == 1 else lam.stride(0),
-                0 if norm_weight is None else norm_weight.data_ptr(),
-                0 if norm_weight is None else _FLOAT_CODES[norm_weight.dtype], float(norm_eps), float(out_scale),
-                out.data_ptr(), _FLOAT_CODES[out.dtype], _lib.i64(out.stride()),
-                splits, ws.data_ptr(), nbytes, status, _stream_ptr(device))
-        if int8:
-            rc = lib.int8kv_paged_diff_attn_int8(*head, *mid, k_scale.data_ptr(), v_scale.data_ptr(), *tail)
-        else:
-            rc = lib.int8kv_paged_diff_attn_bf16(*head, _FLOAT_CODES[key_cache.dtype], *mid, *tail)
-    _lib.check("int8kv_paged_diff_attn_int8" if int8 else "int8kv_paged_diff_attn_bf16", rc)
+    width = block_tables.shape[1]
+    limit = width * block_size
+    nbytes = _workspace_bytes(B, H, P, D, min(max_seq, limit) if max_seq > 0 else limit, block_size, splits, _sm_count(device))
+    # The partial rows belong to the call: memory of the current stream, or of the pool of the graph that captures the
+    # call.  The status word is the stream's, the one that device_status() reads.
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    i64 = _lib.i64
+    rc = _call(
+        device, lib.int8kv_paged_diff_attn_int8 if int8 else lib.int8kv_paged_diff_attn_bf16,
+        query.data_ptr(), q_code, i64(query.stride()), B, H, P, D, key_cache.data_ptr(), value_cache.data_ptr(),
+        *(() if int8 else (_FLOAT_CODES[key_cache.dtype],)),
+        i64(kc_st), i64(vc_st), num_blocks, block_size, block_tables.data_ptr(), bt_code, i64(bt_st), width,
+        seq_lens.data_ptr(), sl_code, max_seq,
+        *((k_scale.data_ptr(), v_scale.data_ptr()) if int8 else ()),
+        lam.data_ptr(), lam_code, 0 if lams == 1 else lam.stride(0), norm_ptr, norm_code, norm_eps, out_scale,
+        out.data_ptr(), out_code, i64(out.stride()), splits, ws.data_ptr(), nbytes, _status_ptr(device),
+    )
+    if rc != _lib.OK:
+        _lib.check("int8kv_paged_diff_attn_int8" if int8 else "int8kv_paged_diff_attn_bf16", rc)
     return out
 
 
@@ -105,8 +120,7 @@ def int8_paged_diff_attention(
     """
     assert key_cache.dtype == torch.int8 and value_cache.dtype == torch.int8
     assert k_scale.device == query.device and v_scale.device == query.device
-    assert k_scale.ndim == 1 and v_scale.ndim == 1
-    assert k_scale.numel() == key_cache.shape[2] and v_scale.numel() == key_cache.shape[2]
+    assert key_cache.ndim == 4 and k_scale.shape == v_scale.shape == key_cache.shape[2:3]
     return _run(True, query, key_cache, value_cache, block_tables, seq_lens, _as_f32_scale(k_scale),
                 _as_f32_scale(v_scale), lam, norm_weight, norm_eps, out_scale, num_splits, max_seq_len, out)
 

@@ -35,8 +35,7 @@ _WS_LOCK = threading.Lock()
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    key = (device.index if device.index is not None else torch.cuda.current_device(),
-           torch.cuda.current_stream(device).cuda_stream)
+    key = (device.index if device.index is not None else torch.cuda.current_device(), _stream_ptr(device))
     with _WS_LOCK:
         buf = _WS.get(key)
         if buf is None or buf.numel() < nbytes:
@@ -91,8 +90,30 @@ def selftest_bounded_wait(attempts: int = 200, device=None) -> int:
     return device_status(device)
 
 
+# The handle of a device's current stream without building a Stream object around it (0.1 us against 3 us per call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    if _raw_stream is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
+
+
+def _status_ptr(device: torch.device) -> int:
+    """Address of the status word that device_status() reads on the device's current stream."""
+    buf = _WS.get((device.index, _stream_ptr(device)))
+    if buf is None:
+        buf = _workspace(device, 16)
+    return buf.data_ptr() + ((buf.numel() - 16) & ~15)
+
+
+def _call(device: torch.device, fn, *args) -> int:
+    """fn(*args, current stream of `device`) with `device` current: a launch goes to the device that its stream is of."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args, _stream_ptr(device))
+    with torch.cuda.device(device):
+        return fn(*args, _stream_ptr(device))
 
 
 def _as_f32_scale(scale: torch.Tensor) -> torch.Tensor:
