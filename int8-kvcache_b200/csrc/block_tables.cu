@@ -6,9 +6,11 @@
 //   first = exclusive prefix sum of want over the requests, granted = want == 0 or first + want <= free entries,
 //   table[old + j] = free[f + first + j],  slot of token i = block(pos / S) * S + pos % S with pos = c + i.
 // Everything hangs on two prefix sums over the requests, so one CTA makes them (plan).  Small calls are bound by launch
-// latency and finish in that CTA, out of its shared memory; larger ones leave 16 bytes per request in the workspace
-// and a second kernel, launched with programmatic dependent launch, writes tables and slots with the whole machine,
-// one 8-byte slot per token being what it cannot do without.
+// latency and by one chain of dependent loads (length -> block id -> slot) and finish in that CTA: a decode step, where
+// every request adds a few tokens, thread by thread with the block id requested before the sums; other small calls
+// out of shared memory.  Larger ones leave 24 bytes per request in the workspace and a second kernel, launched with
+// programmatic dependent launch, writes tables and slots with the whole machine, one 8-byte slot per token being what
+// it cannot do without.
 // All inputs are read before any output is written by the one CTA that reads them, so the new lengths and the cursor
 // may be written over the old ones: a captured step then advances its own state.
 #include <algorithm>
@@ -64,7 +66,8 @@ __device__ __forceinline__ void tab_request(const TableParams& p, int b, int64_t
 
 // Exclusive saturating prefix sums of (x, y) over the CTA's threads, in place; totals in `all`.  (Exclusive by shifting,
 // not by subtraction: a sum that has saturated cannot be undone.)
-__device__ __forceinline__ void tab_scan(uint32_t& x, uint32_t& y, uint32_t* warp_x, uint32_t* warp_y, uint2& all) {
+// Returns whether `vote` held on any thread.
+__device__ __forceinline__ bool tab_scan(uint32_t& x, uint32_t& y, uint32_t* warp_x, uint32_t* warp_y, uint2& all, bool vote) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   auto warp_scan = [lane](uint32_t& a, uint32_t& b) {
     for (int o = 1; o < kWarp; o <<= 1) {
@@ -83,7 +86,7 @@ __device__ __forceinline__ void tab_scan(uint32_t& x, uint32_t& y, uint32_t* war
   x = __shfl_up_sync(kFull, x, 1);
   y = __shfl_up_sync(kFull, y, 1);
   if (lane == 0) x = y = 0u;
-  __syncthreads();
+  const bool any = __syncthreads_or(vote);
   uint32_t a = lane < warps ? warp_x[lane] : 0u, b = lane < warps ? warp_y[lane] : 0u;  // every warp scans the sums
   warp_scan(a, b);
   all = make_uint2(__shfl_sync(kFull, a, kWarp - 1), __shfl_sync(kFull, b, kWarp - 1));
@@ -94,17 +97,33 @@ __device__ __forceinline__ void tab_scan(uint32_t& x, uint32_t& y, uint32_t* war
     x = sat_add(x, a);
     y = sat_add(y, b);
   }
+  return any;
 }
 
-// Last request b in [0, R) with key(b) <= k (key(0) = 0 <= k always).
 template <bool BY_TOKEN>
-__device__ __forceinline__ int tab_owner(const TabRecord* rec, int R, uint32_t k) {
-  int lo = 0, hi = R;  // key(lo) <= k, key(hi) > k or hi == R
+__device__ __forceinline__ uint32_t tab_key(const TabRecord& r) { return BY_TOKEN ? r.start : r.first; }
+
+// Last request b in [lo, hi) with key(b) <= k, where key(lo) <= k.
+template <bool BY_TOKEN>
+__device__ __forceinline__ int tab_owner(const TabRecord* rec, int lo, int hi, uint32_t k) {
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    const uint32_t key = BY_TOKEN ? rec[mid].start : rec[mid].first;
-    if (key <= k) lo = mid;
+    if (tab_key<BY_TOKEN>(rec[mid]) <= k) lo = mid;
     else hi = mid;
+  }
+  return lo;
+}
+
+// The same by a whole warp: 32 probes per round, two rounds for up to 1024 requests.
+template <bool BY_TOKEN>
+__device__ __forceinline__ int tab_owner_warp(const TabRecord* rec, int R, uint32_t k, int lane) {
+  int lo = 0, len = R;
+  while (len > 1) {
+    const int step = (len + kWarp - 1) / kWarp, at = lane * step;
+    const unsigned hit = __ballot_sync(kFull, at < len && (lane == 0 || tab_key<BY_TOKEN>(rec[lo + min(at, len - 1)]) <= k));
+    const int skip = (__popc(hit) - 1) * step;  // the hits are a prefix of the lanes
+    lo += skip;
+    len = min(step, len - skip);
   }
   return lo;
 }
@@ -115,34 +134,33 @@ __device__ __forceinline__ uint32_t tab_room(const TableParams& p, int64_t curso
   return room <= 0 ? 0u : static_cast<uint32_t>(min(room, static_cast<int64_t>(kTabSat - 1)));
 }
 
-__device__ __forceinline__ int64_t tab_slot(const TableParams& p, const TabRecord* rec, const TabTotals& tot, uint32_t tok) {
-  if (tok >= tot.tokens) return -1;
-  const int b = tab_owner<true>(rec, p.R, tok);
+__device__ __forceinline__ int64_t tab_table(const TableParams& p, int b, int64_t j) {
+  return load_index_rw(p.bt, p.bt_is_i64, b * p.bt_st[0] + j * p.bt_st[1]);
+}
+
+// Slot of token `tok` of the packed order, which belongs to request b.
+__device__ __forceinline__ int64_t tab_slot(const TableParams& p, const TabRecord* rec, const TabTotals& tot, int b, uint32_t tok) {
   const TabRecord r = rec[b];
   if (r.cached < 0) return -1;
   const int64_t pos = r.cached + (tok - r.start);
   const int64_t j = div_block(pos, p.block_size);
+  const int64_t begin = j * p.block_size;
   int64_t blk = -1;
-  const int64_t old = p.mode == kTabGrow ? div_block(r.cached + p.block_size - 1, p.block_size) : p.width;
-  if (j < old) blk = load_index_rw(p.bt, p.bt_is_i64, b * p.bt_st[0] + j * p.bt_st[1]);
-  else if (p.mode == kTabGrow) blk = load_index(p.free_blocks, p.free_is_i64, tot.cursor + r.first + (j - old));
-  return blk < 0 ? -1 : blk * p.block_size + (pos - j * p.block_size);
+  if (p.mode == kTabGrow && begin >= r.cached) blk = load_index(p.free_blocks, p.free_is_i64, tot.cursor + j + r.shift);
+  else if (j < p.width) blk = tab_table(p, b, j);
+  return blk < 0 ? -1 : blk * p.block_size + (pos - begin);
 }
 
-// One block that moves: number k in the order of all blocks.
-__device__ __forceinline__ void tab_move(const TableParams& p, const TabRecord* rec, const TabTotals& tot, uint32_t k) {
-  const int b = tab_owner<false>(rec, p.R, k);
+// One block that moves: number k in the order of all blocks, of request b.
+__device__ __forceinline__ void tab_move(const TableParams& p, const TabRecord* rec, const TabTotals& tot, int b, uint32_t k) {
   const TabRecord r = rec[b];
   if (r.cached < 0) return;
+  const int64_t j = static_cast<int64_t>(k) - r.shift;
   if (p.mode == kTabGrow) {
-    const int64_t j = div_block(r.cached + p.block_size - 1, p.block_size) + (k - r.first);
-    store_index(p.bt, p.bt_is_i64, b * p.bt_st[0] + j * p.bt_st[1],
-                load_index(p.free_blocks, p.free_is_i64, tot.cursor + k));
+    store_index(p.bt, p.bt_is_i64, b * p.bt_st[0] + j * p.bt_st[1], load_index(p.free_blocks, p.free_is_i64, tot.cursor + k));
   } else {
     const int64_t at = tot.cursor - tot.blocks + k;
-    if (at >= 0 && at < p.num_free)
-      store_index(p.free_out, p.free_is_i64, at,
-                  load_index_rw(p.bt, p.bt_is_i64, b * p.bt_st[0] + static_cast<int64_t>(k - r.first) * p.bt_st[1]));
+    if (at >= 0 && at < p.num_free) store_index(p.free_out, p.free_is_i64, at, tab_table(p, b, j));
   }
 }
 
@@ -153,10 +171,11 @@ __device__ __forceinline__ uint32_t tab_moves(const TableParams& p, const TabTot
 }
 
 constexpr int kTabThreads = 1024;
+constexpr uint32_t kTabFew = 4;  // new tokens of a request that one thread places by itself
 
 // The prefix sums, the outputs of one value per request, and, when FUSED, the whole write phase.
 template <bool FUSED>
-__global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const TableParams p) {
+__global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const __grid_constant__ TableParams p) {
   extern __shared__ __align__(16) uint8_t tab_smem[];
   __shared__ uint32_t warp_x[kWarp], warp_y[kWarp];
   __shared__ unsigned int taken_s;
@@ -165,48 +184,83 @@ __global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const TablePara
   TabRecord* rec = FUSED ? reinterpret_cast<TabRecord*>(tab_smem) : p.records;
   TabTotals tot;
   tot.cursor = p.mode == kTabSlots ? 0 : *p.cursor;
-  if (tot.cursor < 0) tot.cursor = 0;
-  if (p.mode == kTabRelease && tot.cursor > p.num_free) tot.cursor = p.num_free;
   if (threadIdx.x == 0) taken_s = 0u;
   const int run = (p.R + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
   const int lo = min(static_cast<int>(threadIdx.x) * run, p.R), hi = min(lo + run, p.R);
   uint32_t x = 0, y = 0;
+  int64_t c0 = 0;  // this thread's first request stays in registers
+  uint32_t n0 = 0, want0 = 0;
+  bool fits0 = false;
   for (int b = lo; b < hi; ++b) {
     int64_t c;
     uint32_t n, want;
     bool fits;
     tab_request(p, b, c, n, want, fits);
+    if (b == lo) {
+      c0 = c; n0 = n; want0 = want; fits0 = fits;
+    }
     x = sat_add(x, n);
     y = sat_add(y, want);
   }
+  // A thread's only request with few new tokens: its first block, if the table has it, is requested ahead of the sums.
+  const bool few = FUSED && p.mode != kTabRelease && run <= 1 && n0 <= kTabFew;
+  int64_t j0 = 0, known = -1;
+  int off0 = 0;
+  if (few && lo < hi && n0 > 0) {
+    j0 = div_block(c0, p.block_size);
+    off0 = static_cast<int>(c0 - j0 * p.block_size);
+    if (j0 < p.width && (off0 > 0 || p.mode == kTabSlots)) known = tab_table(p, lo, j0);
+  }
   uint2 all;
-  tab_scan(x, y, warp_x, warp_y, all);
+  const bool some_many = tab_scan(x, y, warp_x, warp_y, all, !few);
+  if (tot.cursor < 0) tot.cursor = 0;
+  if (p.mode == kTabRelease && tot.cursor > p.num_free) tot.cursor = p.num_free;
   tot.tokens = all.x;
   tot.blocks = all.y;
   const uint32_t room = p.mode == kTabGrow ? tab_room(p, tot.cursor) : kTabSat;
-  uint32_t at_x = x, at_y = y;
-  uint32_t taken = 0;
+  uint32_t at_x = x, at_y = y, taken = 0;
   for (int b = lo; b < hi; ++b) {
-    int64_t c;
-    uint32_t n, want;
-    bool fits;
-    tab_request(p, b, c, n, want, fits);
+    int64_t c = c0;
+    uint32_t n = n0, want = want0;
+    bool fits = fits0;
+    if (b != lo) tab_request(p, b, c, n, want, fits);
     const uint32_t end = sat_add(at_y, want);
     TabRecord r;
+    r.cached = c;
     r.start = at_x;
     r.first = at_y;
+    r.shift = static_cast<int32_t>(at_y);  // release: from the row's first block on
     if (p.mode == kTabGrow) {
       const bool granted = fits && (want == 0u || end <= room);
       if (granted && want > 0u) taken = max(taken, end);
-      r.cached = granted ? c : -1;
+      if (!granted) r.cached = -1;
+      // (a refused request's shift is never used; a granted one has c <= width * S, so its block count fits 32 bits)
+      r.shift = static_cast<int32_t>(at_y - static_cast<uint32_t>(div_block(c + p.block_size - 1, p.block_size)));
       store_index(p.lens_out, p.lens_is_i64, b, granted ? c + n : c);
     } else if (p.mode == kTabRelease) {
       r.cached = 0;
       store_index(p.lens_out, p.lens_is_i64, b, p.finished[b] ? 0 : c);
-    } else {
-      r.cached = c;
     }
-    rec[b] = r;
+    if (!FUSED || some_many) {
+      rec[b] = r;
+    } else {  // every request of the call has few tokens: each thread places its own
+      int64_t j = j0, blk = known;
+      int off = off0;
+      for (uint32_t i = 0; i < n; ++i) {
+        if (p.mode == kTabGrow && off == 0 && r.cached >= 0) {
+          blk = load_index(p.free_blocks, p.free_is_i64, tot.cursor + j + r.shift);
+          store_index(p.bt, p.bt_is_i64, b * p.bt_st[0] + j * p.bt_st[1], blk);
+        } else if (p.mode == kTabSlots && off == 0 && i > 0) {
+          blk = j < p.width ? tab_table(p, b, j) : -1;
+        }
+        const uint32_t tok = at_x + i;
+        if (tok < static_cast<uint32_t>(p.num_tokens)) p.slots[tok] = r.cached < 0 || blk < 0 ? -1 : blk * p.block_size + off;
+        if (++off == p.block_size) {
+          off = 0;
+          ++j;
+        }
+      }
+    }
     if (p.query_start != nullptr) p.query_start[b] = static_cast<int32_t>(at_x);
     at_x = sat_add(at_x, n);
     at_y = end;
@@ -214,46 +268,79 @@ __global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const TablePara
   if (p.query_start != nullptr && threadIdx.x == 0) p.query_start[p.R] = static_cast<int32_t>(tot.tokens);
   if (p.mode == kTabGrow && taken > 0u) atomicMax(&taken_s, taken);
   __syncthreads();
-  if (threadIdx.x == 0 && p.mode != kTabSlots) {
-    const int64_t next = p.mode == kTabGrow ? tot.cursor + taken_s : tot.cursor - static_cast<int64_t>(tot.blocks);
-    *p.cursor_out = next < 0 ? 0 : next;
+  if (threadIdx.x == 0) {
+    if (p.mode != kTabSlots) {
+      const int64_t next = p.mode == kTabGrow ? tot.cursor + taken_s : tot.cursor - static_cast<int64_t>(tot.blocks);
+      *p.cursor_out = next < 0 ? 0 : next;
+    }
+    if (!FUSED) *p.totals = tot;
   }
-  if (!FUSED && threadIdx.x == 0) *p.totals = tot;
   if constexpr (FUSED) {
-    const uint32_t moves = tab_moves(p, tot);
-    for (uint32_t k = threadIdx.x; k < moves; k += blockDim.x) tab_move(p, rec, tot, k);
-    for (uint32_t tok = threadIdx.x; tok < static_cast<uint32_t>(p.num_tokens); tok += blockDim.x)
-      p.slots[tok] = tab_slot(p, rec, tot, tok);
+    const uint32_t tokens = static_cast<uint32_t>(p.num_tokens), live = min(tot.tokens, tokens);
+    if (some_many) {
+      const uint32_t moves = tab_moves(p, tot);
+      for (uint32_t k = threadIdx.x; k < moves; k += blockDim.x) tab_move(p, rec, tot, tab_owner<false>(rec, 0, p.R, k), k);
+      for (uint32_t tok = threadIdx.x; tok < live; tok += blockDim.x)
+        p.slots[tok] = tab_slot(p, rec, tot, tab_owner<true>(rec, 0, p.R, tok), tok);
+    }
+    for (uint32_t tok = live + threadIdx.x; tok < tokens; tok += blockDim.x) p.slots[tok] = -1;
   }
 }
 
 constexpr int kTabWriteThreads = 256;
 
-// The write phase with the whole machine: grid-stride over the tokens, then over the blocks that move.
-__global__ void __launch_bounds__(kTabWriteThreads) table_write_kernel(const TableParams p) {
+// The write phase with the whole machine.  A warp takes a run of consecutive tokens (then of blocks that move), finds
+// the requests of its first and last one together, and each lane searches between those: nothing at all inside a long
+// prompt, five steps where every token is another request's.
+__global__ void __launch_bounds__(kTabWriteThreads) table_write_kernel(const __grid_constant__ TableParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const TabTotals tot = *p.totals;
-  const uint32_t step = gridDim.x * kTabWriteThreads;
-  const uint32_t me = blockIdx.x * kTabWriteThreads + threadIdx.x;
-  for (uint32_t tok = me; tok < static_cast<uint32_t>(p.num_tokens); tok += step) p.slots[tok] = tab_slot(p, p.records, tot, tok);
-  const uint32_t moves = tab_moves(p, tot);
-  for (uint32_t k = me; k < moves; k += step) tab_move(p, p.records, tot, k);
+  const int lane = threadIdx.x & 31;
+  const uint32_t warps = gridDim.x * (kTabWriteThreads / kWarp);
+  const uint32_t me = blockIdx.x * (kTabWriteThreads / kWarp) + (threadIdx.x >> 5);
+  // runs of whole 32-item rows; 64 bits: me * per may pass 2^32
+  auto run_of = [&](uint32_t items, uint32_t& lo, uint32_t& hi) {
+    const uint64_t per = (static_cast<uint64_t>(items) + warps * 32ull - 1) / (warps * 32ull) * 32ull;
+    const uint64_t a = me * per, b = a + per;
+    lo = static_cast<uint32_t>(a < items ? a : items);
+    hi = static_cast<uint32_t>(b < items ? b : items);
+  };
+  uint32_t lo, hi;
+  run_of(static_cast<uint32_t>(p.num_tokens), lo, hi);
+  if (lo < hi) {
+    const uint32_t live = min(hi, tot.tokens);
+    int b0 = 0, b1 = 0;
+    if (lo < live) {
+      b0 = tab_owner_warp<true>(p.records, p.R, lo, lane);
+      b1 = tab_owner_warp<true>(p.records, p.R, live - 1, lane);
+    }
+    for (uint32_t tok = lo + lane; tok < hi; tok += kWarp)
+      p.slots[tok] = tok < live ? tab_slot(p, p.records, tot, tab_owner<true>(p.records, b0, b1 + 1, tok), tok) : -1;
+  }
+  run_of(tab_moves(p, tot), lo, hi);
+  if (lo < hi) {
+    const int b0 = tab_owner_warp<false>(p.records, p.R, lo, lane);
+    const int b1 = tab_owner_warp<false>(p.records, p.R, hi - 1, lane);
+    for (uint32_t k = lo + lane; k < hi; k += kWarp) tab_move(p, p.records, tot, tab_owner<false>(p.records, b0, b1 + 1, k), k);
+  }
 }
 
 int64_t table_workspace_bytes(int R) { return static_cast<int64_t>(R) * sizeof(TabRecord) + 32; }
 
-constexpr int kFusedRequests = 2048;  // 32 KB of records in shared memory
+constexpr int kFusedRequests = 1024;  // one request per thread, 24 KB of records in shared memory
 constexpr int64_t kFusedItems = 8192;
 
 bool table_single_launch(int R, int64_t items) { return R <= kFusedRequests && items <= kFusedItems; }
 
 int launch_tables(TableParams p, void* workspace, int64_t items, int sm_count, cudaStream_t stream) {
-  const unsigned threads = p.R <= 256 ? 256u : static_cast<unsigned>(kTabThreads);
-  if (table_single_launch(p.R, items))
+  if (table_single_launch(p.R, items)) {
+    const unsigned threads = p.R <= 256 && items <= 1024 ? 256u : static_cast<unsigned>(kTabThreads);
     return launch_pdl(table_plan_kernel<true>, 1u, threads, p.R * sizeof(TabRecord), stream, p);
+  }
   p.totals = reinterpret_cast<TabTotals*>(workspace);
   p.records = reinterpret_cast<TabRecord*>(static_cast<char*>(workspace) + 32);
+  const unsigned threads = p.R <= 256 ? 256u : static_cast<unsigned>(kTabThreads);
   const int rc = launch_pdl(table_plan_kernel<false>, 1u, threads, 0, stream, p);
   if (rc != INT8KV_OK) return rc;
   const int64_t want = (items + kTabWriteThreads - 1) / kTabWriteThreads;

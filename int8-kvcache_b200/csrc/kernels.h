@@ -188,10 +188,12 @@ int launch_diff_merge(const DiffParams& d, cudaStream_t stream);
 
 // Block tables and slot maps (block_tables.cu).
 // What the write phase needs of a request.
-struct alignas(16) TabRecord {
+struct alignas(8) TabRecord {
   int64_t cached;   // tokens it held; -1: refused or not taking part
   uint32_t start;   // first of its tokens in the packed order (growth, slots)
   uint32_t first;   // first of its blocks in the order of all blocks that move
+  int32_t shift;    // block number k of that order is its logical block k - shift
+  int32_t unused;
 };
 
 struct TabTotals {

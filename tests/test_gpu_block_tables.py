@@ -38,6 +38,10 @@ CASES = [  # requests, width, block size, lo, hi, new_hi, spare
     (64, 40, 16, 1, 600, 30, 0),
     (255, 17, 7, 0, 100, 15, 2),
     (256, 33, 16, 0, 500, 1, -3),      # the list runs out
+    (300, 25, 1, 0, 20, 4, -20),       # a block per token, a few tokens each, the list runs out
+    (1000, 9, 16, 0, 143, 4, 0),       # a few tokens each, some beyond their row
+    (1, 600, 16, 0, 0, 9000, 3),       # one prompt
+    (3, 300, 64, 100, 9000, 9000, 0),
     (257, 12, 32, 0, 384, 200, 0),     # rows that some requests do not fit
     (1025, 20, 24, 0, 400, 80, -40),   # more requests than threads, the list runs out, the two-kernel form
     (2049, 6, 16, 0, 80, 2, 1),        # more requests than the one-kernel form takes
