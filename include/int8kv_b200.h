@@ -400,12 +400,13 @@ int int8kv_paged_diff_attn_bf16(const void* query, int q_dtype, const int64_t q_
  * rows, seq_lens clamped to what a row holds) go back below the cursor, in request order, and their lengths become 0;
  * the table is not written.  Entries that would lie below position 0 (more blocks given back than were handed out) are
  * dropped.  In-place outputs as above.
- * workspace: int8kv_block_tables_workspace_bytes(num_requests, items) bytes, 16-byte aligned; 0 (and a null workspace)
- * for calls that run as one kernel.  items is an upper bound of the slots and blocks a call writes: num_tokens +
+ * workspace: int8kv_block_tables_workspace_bytes(num_requests, items, in_place) bytes, 16-byte aligned; 0 (and a null
+ * workspace) for calls that run as one kernel.  in_place: whether an output is the input of the same name (never for
+ * a slot mapping).  items is an upper bound of the slots and blocks a call writes: num_tokens +
  * num_tokens / S + num_requests for a growth, num_tokens for a slot mapping, min(num_requests * bt_width, num_free)
  * for a release.
  */
-int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items);
+int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items, int in_place);
 
 int int8kv_build_block_tables(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
                               int num_requests, int block_size,

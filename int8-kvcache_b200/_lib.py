@@ -136,7 +136,7 @@ _SIGNATURES = {
          _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64, _VP, C.c_int, C.c_int64,
          _VP, C.c_int, C.c_float, C.c_float, _VP, C.c_int, _I64P, C.c_int, _VP, C.c_int64, _VP, _VP],
     ),
-    "int8kv_block_tables_workspace_bytes": (C.c_int64, [C.c_int, C.c_int64]),
+    "int8kv_block_tables_workspace_bytes": (C.c_int64, [C.c_int, C.c_int64, C.c_int]),
     "int8kv_build_block_tables": (
         C.c_int,
         [_VP, C.c_int, _VP, C.c_int, C.c_int, C.c_int, _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64,

@@ -14,6 +14,7 @@ captured in a CUDA graph.  The reference builds both on the host (tests/test_int
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -55,10 +56,15 @@ def _check_out(out, device, shape, dtype):
     assert out.shape == shape and out.dtype == dtype and out.device == device and out.is_contiguous()
 
 
-def _workspace(lib, requests: int, items: int, device) -> Tuple[Optional[torch.Tensor], int, int]:
+@lru_cache(maxsize=1024)
+def _workspace_bytes(requests: int, items: int, in_place: bool) -> int:
+    return _require_lib().int8kv_block_tables_workspace_bytes(requests, items, in_place)
+
+
+def _workspace(requests: int, items: int, in_place: bool, device) -> Tuple[Optional[torch.Tensor], int, int]:
     """(tensor, address, bytes) of a call's workspace.  It belongs to the call: a captured call gets memory of its
     graph's own pool, so two graphs never share it."""
-    nbytes = lib.int8kv_block_tables_workspace_bytes(requests, items)
+    nbytes = _workspace_bytes(requests, items, in_place)
     if nbytes <= 0:
         return None, 0, 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -101,13 +107,16 @@ def build_block_tables(
         _check_out(out.free_cursor, device, (1,), torch.int64)
     lib = _require_lib()
     seq_lens, new_lens, free_blocks = seq_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
-    ws, ws_ptr, ws_bytes = _workspace(lib, R, num_tokens + num_tokens // block_size + R, device)
+    lens_ptr, new_ptr, lens_out = seq_lens.data_ptr(), new_lens.data_ptr(), out.seq_lens.data_ptr()
+    cursor_ptr, cursor_out = free_cursor.data_ptr(), out.free_cursor.data_ptr()
+    in_place = lens_out == lens_ptr or lens_out == new_ptr or cursor_ptr == cursor_out
+    ws, ws_ptr, ws_bytes = _workspace(R, num_tokens + num_tokens // block_size + R, in_place, device)
     rc = _call(
         device, lib.int8kv_build_block_tables,
-        seq_lens.data_ptr(), sl_code, new_lens.data_ptr(), nl_code, R, block_size,
+        lens_ptr, sl_code, new_ptr, nl_code, R, block_size,
         block_tables.data_ptr(), bt_code, _lib.i64(bt_st), width,
         free_blocks.data_ptr(), fb_code, free_blocks.shape[0],
-        free_cursor.data_ptr(), out.free_cursor.data_ptr(), out.seq_lens.data_ptr(),
+        cursor_ptr, cursor_out, lens_out,
         out.slot_mapping.data_ptr(), num_tokens, out.query_start.data_ptr(), ws_ptr, ws_bytes,
     )
     if rc != _lib.OK:
@@ -139,7 +148,7 @@ def build_slot_mapping(
         _check_out(out[1], device, (R + 1,), torch.int32)
     lib = _require_lib()
     seq_lens, new_lens = seq_lens.contiguous(), new_lens.contiguous()
-    ws, ws_ptr, ws_bytes = _workspace(lib, R, num_tokens, device)
+    ws, ws_ptr, ws_bytes = _workspace(R, num_tokens, False, device)
     rc = _call(
         device, lib.int8kv_build_slot_mapping,
         seq_lens.data_ptr(), sl_code, new_lens.data_ptr(), nl_code, R, block_size,
@@ -177,13 +186,15 @@ def release_block_tables(
     lib = _require_lib()
     seq_lens, finished = seq_lens.contiguous(), finished.contiguous()
     N = free_blocks.shape[0]
-    ws, ws_ptr, ws_bytes = _workspace(lib, R, min(R * width, N), device)
+    lens_ptr, lens_out, cursor_ptr, cursor_out = (
+        seq_lens.data_ptr(), out[0].data_ptr(), free_cursor.data_ptr(), out[1].data_ptr())
+    ws, ws_ptr, ws_bytes = _workspace(R, min(R * width, N), lens_ptr == lens_out or cursor_ptr == cursor_out, device)
     rc = _call(
         device, lib.int8kv_release_block_tables,
-        seq_lens.data_ptr(), sl_code, finished.data_ptr(), R, block_size,
+        lens_ptr, sl_code, finished.data_ptr(), R, block_size,
         block_tables.data_ptr(), bt_code, _lib.i64(block_tables.stride()), width,
         free_blocks.data_ptr(), fb_code, N,
-        free_cursor.data_ptr(), out[1].data_ptr(), out[0].data_ptr(), ws_ptr, ws_bytes,
+        cursor_ptr, cursor_out, lens_out, ws_ptr, ws_bytes,
     )
     if rc != _lib.OK:
         _lib.check("int8kv_release_block_tables", rc)

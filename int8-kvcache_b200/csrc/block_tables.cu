@@ -5,14 +5,16 @@
 //   old = ceil(c / S), want = ceil((c + n) / S) - old (0 and refused when c + n > W * S),
 //   first = exclusive prefix sum of want over the requests, granted = want == 0 or first + want <= free entries,
 //   table[old + j] = free[f + first + j],  slot of token i = block(pos / S) * S + pos % S with pos = c + i.
-// Everything hangs on two prefix sums over the requests, so one CTA makes them (plan).  Small calls are bound by launch
-// latency and by one chain of dependent loads (length -> block id -> slot) and finish in that CTA: a decode step, where
-// every request adds a few tokens, thread by thread with the block id requested before the sums; other small calls
-// out of shared memory.  Larger ones leave 24 bytes per request in the workspace and a second kernel, launched with
-// programmatic dependent launch, writes tables and slots with the whole machine, one 8-byte slot per token being what
-// it cannot do without.
-// All inputs are read before any output is written by the one CTA that reads them, so the new lengths and the cursor
-// may be written over the old ones: a captured step then advances its own state.
+// Everything hangs on two prefix sums over the requests.  A CTA makes them in about a microsecond out of L2, so every
+// CTA of the launch makes them for itself and then writes its share of slots and blocks: one launch, no workspace, no
+// pass over intermediate records.  Small calls are one CTA, bound by launch latency and one chain of dependent
+// loads (length -> block id -> slot); a decode step, where every request adds a few tokens, goes thread by thread with
+// the block id requested ahead of the sums.  Large ones are bound by the 8 bytes per slot that they write.
+// With many requests, or when a large call's new lengths or cursor are to be written over the old ones (which other
+// CTAs may still be reading), one CTA makes the sums, leaves 24 bytes per request in the workspace, and a second kernel,
+// launched with programmatic dependent launch, writes slots and blocks.
+// The CTA that writes the new lengths and the cursor has read the old ones by then, so they may be the same memory: a
+// captured step then advances its own state.
 #include <algorithm>
 
 #include "common.cuh"
@@ -170,10 +172,66 @@ __device__ __forceinline__ uint32_t tab_moves(const TableParams& p, const TabTot
   return p.mode == kTabGrow ? min(tot.blocks, tab_room(p, tot.cursor)) : tot.blocks;
 }
 
+// The write phase of warp `me` of `warps`: a run of consecutive tokens, then one of blocks that move.  The warp finds the
+// requests of the run's first and last item together.  Mostly they are the same (a prompt): then everything but the
+// position is uniform.  Otherwise each lane searches between them, five steps where every token is another
+// request's.
+__device__ __forceinline__ void tab_run(uint32_t items, uint32_t me, uint32_t warps, uint32_t& lo, uint32_t& hi) {
+  const uint32_t rows = (items >> 5) + 1, per = (rows + warps - 1) / warps;  // rows of 32 items, per warp
+  const uint64_t a = static_cast<uint64_t>(me) * per * 32u, b = a + per * 32ull;
+  lo = static_cast<uint32_t>(a < items ? a : items);
+  hi = static_cast<uint32_t>(b < items ? b : items);
+}
+
+__device__ __forceinline__ void tab_write_slots(const TableParams& p, const TabRecord* rec, const TabTotals& tot, uint32_t me,
+                                                uint32_t warps, int lane) {
+  uint32_t lo, hi;
+  tab_run(static_cast<uint32_t>(p.num_tokens), me, warps, lo, hi);
+  const uint32_t live = min(hi, tot.tokens);
+  if (lo < live) {
+    const int b0 = tab_owner_warp<true>(rec, p.R, lo, lane);
+    const int b1 = tab_owner_warp<true>(rec, p.R, live - 1, lane);
+    const TabRecord r = rec[b0];
+    if (b0 == b1 && r.cached >= 0 && r.cached + (live - r.start) <= 0xffffffffll && p.width <= 0x7fffffffll) {
+      const uint32_t S = p.block_size, cached = static_cast<uint32_t>(r.cached), p0 = cached - r.start;
+      const bool grow = p.mode == kTabGrow;
+      const uint32_t width = static_cast<uint32_t>(p.width);
+      const int64_t row = b0 * p.bt_st[0], list = tot.cursor + r.shift;
+#pragma unroll 4
+      for (uint32_t tok = lo + lane; tok < live; tok += kWarp) {
+        const uint32_t pos = p0 + tok;
+        const uint32_t j = p.block_shift >= 0 ? pos >> p.block_shift : pos / S;
+        const uint32_t begin = j * S;
+        int64_t blk = -1;
+        if (grow && begin >= cached) blk = load_index(p.free_blocks, p.free_is_i64, list + j);
+        else if (j < width) blk = load_index_rw(p.bt, p.bt_is_i64, row + j * p.bt_st[1]);
+        p.slots[tok] = blk < 0 ? -1 : blk * S + (pos - begin);
+      }
+    } else {
+      for (uint32_t tok = lo + lane; tok < live; tok += kWarp)
+        p.slots[tok] = tab_slot(p, rec, tot, tab_owner<true>(rec, b0, b1 + 1, tok), tok);
+    }
+  }
+  for (uint32_t tok = max(lo, live) + lane; tok < hi; tok += kWarp) p.slots[tok] = -1;
+}
+
+__device__ __forceinline__ void tab_write_moves(const TableParams& p, const TabRecord* rec, const TabTotals& tot, uint32_t me,
+                                                uint32_t warps, int lane) {
+  uint32_t lo, hi;
+  tab_run(tab_moves(p, tot), me, warps, lo, hi);
+  if (lo >= hi) return;
+  const int b0 = tab_owner_warp<false>(rec, p.R, lo, lane);
+  const int b1 = tab_owner_warp<false>(rec, p.R, hi - 1, lane);
+#pragma unroll 4
+  for (uint32_t k = lo + lane; k < hi; k += kWarp)
+    tab_move(p, rec, tot, b0 == b1 ? b0 : tab_owner<false>(rec, b0, b1 + 1, k), k);
+}
+
 constexpr int kTabThreads = 1024;
 constexpr uint32_t kTabFew = 4;  // new tokens of a request that one thread places by itself
 
-// The prefix sums, the outputs of one value per request, and, when FUSED, the whole write phase.
+// The prefix sums, the outputs of one value per request (CTA 0), and, when FUSED, this CTA's share of the write phase.
+// More than one CTA only when no output is an input.
 template <bool FUSED>
 __global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const __grid_constant__ TableParams p) {
   extern __shared__ __align__(16) uint8_t tab_smem[];
@@ -182,6 +240,7 @@ __global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const __grid_co
   grid_dependency_wait();
   grid_launch_dependents();
   TabRecord* rec = FUSED ? reinterpret_cast<TabRecord*>(tab_smem) : p.records;
+  const bool first_cta = blockIdx.x == 0;
   TabTotals tot;
   tot.cursor = p.mode == kTabSlots ? 0 : *p.cursor;
   if (threadIdx.x == 0) taken_s = 0u;
@@ -236,14 +295,14 @@ __global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const __grid_co
       if (!granted) r.cached = -1;
       // (a refused request's shift is never used; a granted one has c <= width * S, so its block count fits 32 bits)
       r.shift = static_cast<int32_t>(at_y - static_cast<uint32_t>(div_block(c + p.block_size - 1, p.block_size)));
-      store_index(p.lens_out, p.lens_is_i64, b, granted ? c + n : c);
+      if (first_cta) store_index(p.lens_out, p.lens_is_i64, b, granted ? c + n : c);
     } else if (p.mode == kTabRelease) {
       r.cached = 0;
-      store_index(p.lens_out, p.lens_is_i64, b, p.finished[b] ? 0 : c);
+      if (first_cta) store_index(p.lens_out, p.lens_is_i64, b, p.finished[b] ? 0 : c);
     }
     if (!FUSED || some_many) {
       rec[b] = r;
-    } else {  // every request of the call has few tokens: each thread places its own
+    } else if (first_cta) {  // every request of the call has few tokens: each thread places its own
       int64_t j = j0, blk = known;
       int off = off0;
       for (uint32_t i = 0; i < n; ++i) {
@@ -261,14 +320,14 @@ __global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const __grid_co
         }
       }
     }
-    if (p.query_start != nullptr) p.query_start[b] = static_cast<int32_t>(at_x);
+    if (first_cta && p.query_start != nullptr) p.query_start[b] = static_cast<int32_t>(at_x);
     at_x = sat_add(at_x, n);
     at_y = end;
   }
-  if (p.query_start != nullptr && threadIdx.x == 0) p.query_start[p.R] = static_cast<int32_t>(tot.tokens);
+  if (first_cta && p.query_start != nullptr && threadIdx.x == 0) p.query_start[p.R] = static_cast<int32_t>(tot.tokens);
   if (p.mode == kTabGrow && taken > 0u) atomicMax(&taken_s, taken);
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (first_cta && threadIdx.x == 0) {
     if (p.mode != kTabSlots) {
       const int64_t next = p.mode == kTabGrow ? tot.cursor + taken_s : tot.cursor - static_cast<int64_t>(tot.blocks);
       *p.cursor_out = next < 0 ? 0 : next;
@@ -276,22 +335,21 @@ __global__ void __launch_bounds__(kTabThreads) table_plan_kernel(const __grid_co
     if (!FUSED) *p.totals = tot;
   }
   if constexpr (FUSED) {
-    const uint32_t tokens = static_cast<uint32_t>(p.num_tokens), live = min(tot.tokens, tokens);
+    const int lane = threadIdx.x & 31;
+    const uint32_t warps = gridDim.x * (blockDim.x >> 5), me = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (some_many) {
-      const uint32_t moves = tab_moves(p, tot);
-      for (uint32_t k = threadIdx.x; k < moves; k += blockDim.x) tab_move(p, rec, tot, tab_owner<false>(rec, 0, p.R, k), k);
-      for (uint32_t tok = threadIdx.x; tok < live; tok += blockDim.x)
-        p.slots[tok] = tab_slot(p, rec, tot, tab_owner<true>(rec, 0, p.R, tok), tok);
+      tab_write_moves(p, rec, tot, me, warps, lane);
+      tab_write_slots(p, rec, tot, me, warps, lane);
+    } else {
+      const uint32_t tokens = static_cast<uint32_t>(p.num_tokens);
+      for (uint32_t tok = min(tot.tokens, tokens) + me * kWarp + lane; tok < tokens; tok += warps * kWarp) p.slots[tok] = -1;
     }
-    for (uint32_t tok = live + threadIdx.x; tok < tokens; tok += blockDim.x) p.slots[tok] = -1;
   }
 }
 
 constexpr int kTabWriteThreads = 256;
 
-// The write phase with the whole machine.  A warp takes a run of consecutive tokens (then of blocks that move), finds
-// the requests of its first and last one together, and each lane searches between those: nothing at all inside a long
-// prompt, five steps where every token is another request's.
+// The write phase of a call whose sums another kernel has left in the workspace.
 __global__ void __launch_bounds__(kTabWriteThreads) table_write_kernel(const __grid_constant__ TableParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
@@ -299,48 +357,30 @@ __global__ void __launch_bounds__(kTabWriteThreads) table_write_kernel(const __g
   const int lane = threadIdx.x & 31;
   const uint32_t warps = gridDim.x * (kTabWriteThreads / kWarp);
   const uint32_t me = blockIdx.x * (kTabWriteThreads / kWarp) + (threadIdx.x >> 5);
-  // runs of whole 32-item rows; 64 bits: me * per may pass 2^32
-  auto run_of = [&](uint32_t items, uint32_t& lo, uint32_t& hi) {
-    const uint64_t per = (static_cast<uint64_t>(items) + warps * 32ull - 1) / (warps * 32ull) * 32ull;
-    const uint64_t a = me * per, b = a + per;
-    lo = static_cast<uint32_t>(a < items ? a : items);
-    hi = static_cast<uint32_t>(b < items ? b : items);
-  };
-  uint32_t lo, hi;
-  run_of(static_cast<uint32_t>(p.num_tokens), lo, hi);
-  if (lo < hi) {
-    const uint32_t live = min(hi, tot.tokens);
-    int b0 = 0, b1 = 0;
-    if (lo < live) {
-      b0 = tab_owner_warp<true>(p.records, p.R, lo, lane);
-      b1 = tab_owner_warp<true>(p.records, p.R, live - 1, lane);
-    }
-    for (uint32_t tok = lo + lane; tok < hi; tok += kWarp)
-      p.slots[tok] = tok < live ? tab_slot(p, p.records, tot, tab_owner<true>(p.records, b0, b1 + 1, tok), tok) : -1;
-  }
-  run_of(tab_moves(p, tot), lo, hi);
-  if (lo < hi) {
-    const int b0 = tab_owner_warp<false>(p.records, p.R, lo, lane);
-    const int b1 = tab_owner_warp<false>(p.records, p.R, hi - 1, lane);
-    for (uint32_t k = lo + lane; k < hi; k += kWarp) tab_move(p, p.records, tot, tab_owner<false>(p.records, b0, b1 + 1, k), k);
-  }
+  tab_write_moves(p, p.records, tot, me, warps, lane);
+  tab_write_slots(p, p.records, tot, me, warps, lane);
 }
 
 int64_t table_workspace_bytes(int R) { return static_cast<int64_t>(R) * sizeof(TabRecord) + 32; }
 
-constexpr int kFusedRequests = 1024;  // one request per thread, 24 KB of records in shared memory
-constexpr int64_t kFusedItems = 8192;
+constexpr int kFusedRequests = kTabThreads;  // one request per thread, 24 KB of records in shared memory
+constexpr int64_t kOneCtaItems = 4096;       // slots and blocks that one CTA writes faster than a second launch starts
 
-bool table_single_launch(int R, int64_t items) { return R <= kFusedRequests && items <= kFusedItems; }
+bool table_single_launch(const TableParams& p, int64_t items) {
+  if (p.R > kFusedRequests) return false;
+  return items <= kOneCtaItems || p.mode == kTabSlots || (p.lens_out != p.lens && p.lens_out != p.new_lens && p.cursor_out != p.cursor);
+}
 
 int launch_tables(TableParams p, void* workspace, int64_t items, int sm_count, cudaStream_t stream) {
-  if (table_single_launch(p.R, items)) {
-    const unsigned threads = p.R <= 256 && items <= 1024 ? 256u : static_cast<unsigned>(kTabThreads);
-    return launch_pdl(table_plan_kernel<true>, 1u, threads, p.R * sizeof(TabRecord), stream, p);
+  p.block_shift = (p.block_size & (p.block_size - 1)) == 0 ? 31 - __builtin_clz(static_cast<unsigned>(p.block_size)) : -1;
+  const unsigned threads = p.R <= 256 && items <= 1024 ? 256u : static_cast<unsigned>(kTabThreads);
+  if (table_single_launch(p, items)) {
+    // the registers hold one such CTA per SM
+    const int64_t ctas = items <= kOneCtaItems ? 1 : std::min<int64_t>((items + kTabThreads - 1) / kTabThreads, sm_count);
+    return launch_pdl(table_plan_kernel<true>, static_cast<unsigned>(ctas), threads, p.R * sizeof(TabRecord), stream, p);
   }
   p.totals = reinterpret_cast<TabTotals*>(workspace);
   p.records = reinterpret_cast<TabRecord*>(static_cast<char*>(workspace) + 32);
-  const unsigned threads = p.R <= 256 ? 256u : static_cast<unsigned>(kTabThreads);
   const int rc = launch_pdl(table_plan_kernel<false>, 1u, threads, 0, stream, p);
   if (rc != INT8KV_OK) return rc;
   const int64_t want = (items + kTabWriteThreads - 1) / kTabWriteThreads;

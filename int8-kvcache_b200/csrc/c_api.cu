@@ -1013,7 +1013,7 @@ int table_params(TableParams& p, int mode, const void* lens, int lens_is_i64, in
 }
 
 int run_tables(const TableParams& p, int64_t items, void* ws, int64_t ws_size, void* stream) {
-  const int64_t need = table_single_launch(p.R, items) ? 0 : table_workspace_bytes(p.R);
+  const int64_t need = table_single_launch(p, items) ? 0 : table_workspace_bytes(p.R);
   if (need > 0 && (ws == nullptr || ws_size < need || (reinterpret_cast<uintptr_t>(ws) & 15u))) return INT8KV_E_WORKSPACE;
   return launch_tables(p, ws, items, device_sm_count(), static_cast<cudaStream_t>(stream));
 }
@@ -1022,9 +1022,17 @@ int run_tables(const TableParams& p, int64_t items, void* ws, int64_t ws_size, v
 
 extern "C" {
 
-int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items) {
+int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items, int in_place) {
   if (num_requests < 0 || items < 0) return -1;
-  return table_single_launch(num_requests, items) ? 0 : table_workspace_bytes(num_requests);
+  TableParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.mode = kTabGrow;
+  p.R = num_requests;
+  if (!in_place) {  // outputs that are no inputs
+    p.lens_out = &p;
+    p.cursor_out = reinterpret_cast<int64_t*>(&p);
+  }
+  return table_single_launch(p, items) ? 0 : table_workspace_bytes(num_requests);
 }
 
 int int8kv_build_block_tables(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,

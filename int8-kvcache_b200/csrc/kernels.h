@@ -207,6 +207,7 @@ enum TableMode { kTabGrow = 0, kTabSlots = 1, kTabRelease = 2 };
 struct TableParams {
   int mode;
   int R, block_size;
+  int block_shift;        // log2(block_size), or -1
   int64_t width;          // table columns
   void* bt;               // [R, width]: read, and written by a growth
   int bt_is_i64;
@@ -231,8 +232,8 @@ struct TableParams {
 };
 
 int64_t table_workspace_bytes(int R);
-// Whether a call of R requests with at most `items` slots and moved blocks runs as one kernel, without a workspace.
-bool table_single_launch(int R, int64_t items);
+// Whether a call with at most `items` slots and moved blocks runs as one kernel, without a workspace.
+bool table_single_launch(const TableParams& p, int64_t items);
 int launch_tables(TableParams p, void* workspace, int64_t items, int sm_count, cudaStream_t stream);
 
 int launch_cache_write(const WriteParams& p, int sm_count, cudaStream_t stream);

@@ -44,8 +44,8 @@ def test_c_abi_argument_checks():
     st = lm.i64((4, 1))
     p = C.c_void_p(256)  # never dereferenced: every call below is refused
 
-    def build(R=2, bs=16, width=4, free=8, tokens=4, lens=p, bt=p, cursor=p, start=p, slots=p, ws=None, ws_bytes=0):
-        return lib.int8kv_build_block_tables(lens, 0, p, 0, R, bs, bt, 0, st, width, p, 0, free, cursor, cursor, p,
+    def build(R=2, bs=16, width=4, free=8, tokens=4, lens=p, lens_out=p, bt=p, cursor=p, start=p, slots=p, ws=None, ws_bytes=0):
+        return lib.int8kv_build_block_tables(lens, 0, p, 0, R, bs, bt, 0, st, width, p, 0, free, cursor, cursor, lens_out,
                                              slots, tokens, start, ws, ws_bytes, None)
 
     assert build(R=-1) == lm.E_BAD_SHAPE and build(bs=0) == lm.E_BAD_SHAPE and build(width=-1) == lm.E_BAD_SHAPE
@@ -54,12 +54,14 @@ def test_c_abi_argument_checks():
     assert build(lens=None) == lm.E_NULLPTR and build(bt=None) == lm.E_NULLPTR and build(cursor=None) == lm.E_NULLPTR
     assert build(start=None) == lm.E_NULLPTR and build(slots=None) == lm.E_NULLPTR
     big = 1 << 20
-    need = lib.int8kv_block_tables_workspace_bytes(2, big + big // 16 + 2)
+    need = lib.int8kv_block_tables_workspace_bytes(2, big + big // 16 + 2, 1)
     assert need > 0 and build(tokens=big) == lm.E_WORKSPACE
     assert build(tokens=big, ws=p, ws_bytes=need - 1) == lm.E_WORKSPACE
     assert build(tokens=big, ws=C.c_void_p(264), ws_bytes=need) == lm.E_WORKSPACE
-    assert lib.int8kv_block_tables_workspace_bytes(64, 128) == 0
-    assert lib.int8kv_block_tables_workspace_bytes(-1, 128) == -1
+    assert lib.int8kv_block_tables_workspace_bytes(64, 128, 1) == 0  # small: one kernel
+    assert lib.int8kv_block_tables_workspace_bytes(64, 1 << 20, 0) == 0  # outputs of its own: one kernel of many CTAs
+    assert lib.int8kv_block_tables_workspace_bytes(5000, 128, 0) > 0
+    assert lib.int8kv_block_tables_workspace_bytes(-1, 128, 0) == -1
     assert lib.int8kv_build_slot_mapping(p, 0, None, 0, 2, 16, p, 0, st, 4, p, 4, p, None, 0, None) == lm.E_NULLPTR
     assert lib.int8kv_build_slot_mapping(p, 0, p, 0, 2, 0, p, 0, st, 4, p, 4, p, None, 0, None) == lm.E_BAD_SHAPE
     assert lib.int8kv_release_block_tables(p, 0, None, 2, 16, p, 0, st, 4, p, 0, 8, p, p, p, None, 0, None) == lm.E_NULLPTR
