@@ -92,8 +92,7 @@ static int64_t pow2_floor(int64_t x) {
 // latency-driven count is capped at 16 parts (measured on the 8 x 4096-token cell, per layer: 32 parts 11.1 us, of
 // which the second round trip of the merge is about 2 us) and the rule that cuts the smallest calls into more,
 // shorter parts is left out.
-int choose_splits(int B, int Hkv, int64_t max_seq, int block_size, int sm_count, bool chained = false,
-                  int warps_per_sm = 12) {
+int choose_splits(int B, int Hkv, int64_t max_seq, int block_size, int sm_count, bool chained = false) {
   (void)block_size;
   if (B <= 0 || Hkv <= 0 || max_seq <= 0) return 1;
   const int64_t tiles = (max_seq + 15) / 16;
@@ -104,7 +103,7 @@ int choose_splits(int B, int Hkv, int64_t max_seq, int block_size, int sm_count,
   //    warps, down to 2 tiles per part for short sequences (16 parts) and 8 tiles per part for long ones;
   //  * large calls are bound by HBM, where ragged batches balance best with about four waves of warps, but a part
   //    of fewer than 32 tiles would spend too much of its traffic on its partial rows.
-  const int64_t slots = static_cast<int64_t>(sm_count) * warps_per_sm;
+  const int64_t slots = static_cast<int64_t>(sm_count) * 12;
   const int64_t by_latency = chained ? std::min<int64_t>(tiles / 2, 16)
                                      : std::min<int64_t>(tiles / 2, std::max<int64_t>(16, tiles / 8));
   int64_t s_fill = std::min(pow2_floor(std::max<int64_t>(1, slots / items)), pow2_floor(std::max<int64_t>(1, by_latency)));
@@ -157,22 +156,22 @@ int env_int_or(const char* name, int fallback) {
 // Whether the shape can be planned at all: every warp walks seq_lens a few times, which stays cheap up to a few
 // hundred sequences, and one part per (sequence, head) must fit one wave.
 constexpr int kPlanMaxBatch = 512;
-bool plan_possible(int B, int Hkv, int sm_count, int warps_per_sm = 12) {
-  return B <= kPlanMaxBatch && static_cast<int64_t>(B) * Hkv <= static_cast<int64_t>(sm_count) * warps_per_sm;
+bool plan_possible(int B, int Hkv, int sm_count) {
+  return B <= kPlanMaxBatch && static_cast<int64_t>(B) * Hkv <= static_cast<int64_t>(sm_count) * 12;
 }
 
 // Whether planning pays: enough nominal work for one wave of parts of at least 12 tiles, and a split
 // heuristic that could not reach four waves of warps for this shape (with four or more waves the tail is small and
 // the plan's longer prologue, every warp reading seq_lens before its block table, costs more than it gains:
 // measured 222 us against 216 us per call on the 256-sequence ragged batch).
-bool plan_pays(int B, int Hkv, int64_t max_seq, int block_size, int sm_count, int warps_per_sm = 12) {
+bool plan_pays(int B, int Hkv, int64_t max_seq, int block_size, int sm_count) {
   static const int enabled = env_int_or("INT8KV_PLAN", 1);
-  if (!enabled || !plan_possible(B, Hkv, sm_count, warps_per_sm)) return false;
-  const int64_t slots = static_cast<int64_t>(sm_count) * warps_per_sm;
+  if (!enabled || !plan_possible(B, Hkv, sm_count)) return false;
+  const int64_t slots = static_cast<int64_t>(sm_count) * 12;
   const int64_t items = static_cast<int64_t>(B) * Hkv;
   const int64_t tiles = (max_seq + 15) / 16;
   if (items * tiles < slots * 12) return false;
-  return items * choose_splits(B, Hkv, max_seq, block_size, sm_count, false, warps_per_sm) < slots * 4;
+  return items * choose_splits(B, Hkv, max_seq, block_size, sm_count) < slots * 4;
 }
 
 // Warps per SM that a plan counts as one wave.  A single call fills the machine exactly (12 resident warps per SM).
@@ -1097,39 +1096,41 @@ int int8kv_release_block_tables(const void* seq_lens, int sl_is_i64, const uint8
 // =============================================================================================================
 namespace {
 
-// How a call is cut, decided from its shape alone.
-struct DiffPlan {
-  bool planned;      // parts planned on the device from the lengths
-  int S;             // parts per sequence otherwise
-  PlanShape ps;
-  int64_t table_off; // planned: offset of the sequence table behind the partial rows
-  int64_t need;      // workspace bytes
-};
+int64_t diff_rows_bytes(int64_t rows, int D) { return std::max<int64_t>(rows * partial_row_floats(2 * D) * 4, 16); }
 
-int64_t diff_rows_bytes(int64_t rows, int D) { return rows * partial_row_floats(2 * D) * 4; }
-
-// tiled: the TMA-tiled kernels serve the shape; they split as the ordinary tiled ones do, on the warps that an SM holds of
-// them.  Otherwise one item per query pair, see untiled_splits.
-DiffPlan diff_plan(bool tiled, int cache_kind, int B, int heads, int pairs, int D, int64_t max_seq, int64_t cap, int block_size,
-                   int num_splits, int sm) {
-  DiffPlan t;
-  std::memset(&t, 0, sizeof(t));
-  const int64_t tiles = (max_seq + 15) / 16;
-  const int wps = diff_warps_per_sm(cache_kind, D, heads / pairs);
-  t.planned = tiled && num_splits == 0 && tiles > 0 && cap < (int64_t(1) << 21) * 16 &&
-              plan_pays(B, pairs, max_seq, block_size, sm, wps);
-  if (t.planned) {
-    t.ps = plan_shape(B, pairs, tiles, sm, wps);
-    t.S = kMaxSplits;  // upper bound of the parts of one sequence
-    t.table_off = diff_rows_bytes(static_cast<int64_t>(t.ps.max_items) * 2 * (heads / pairs), D);
-    t.need = t.table_off + static_cast<int64_t>(B) * 8;
-    return t;
+// Parts per sequence of the TMA-tiled kernels, measured on B200.  A part costs its two rows per query pair, written and
+// read again, a prologue and an epilogue; P = tiles of the longest sequence's parts.
+//  * Small calls are bound by one warp's chain of dependent steps, 0.7 us per tile as long as every warp has a scheduler
+//    to itself: four items per SM, parts down to two tiles, and whole batches of 32 parts, which the join takes at a time.
+//    (8 x 4096 tokens over two KV pairs, groups of seven: 8 / 16 / 32 / 37 / 64 parts, 1 to 7 warps per SM, take
+//    32.2 / 21.2 / 18.7 / 19.4 / 22.8 us.)
+//  * From P = 48 on, one resident wave, less one item per SM: with every register taken, the last items wait for a
+//    scheduler's share to come free (32 x 8192 tokens, D = 64, groups of eight: 7 / 8 items per SM 57 / 60 us).
+//  * Large calls are bound by HBM and even out over several waves, as long as the rows stay around 3 % of the K and V
+//    bytes: P = 16 group for INT8, half that for two-byte caches.  (32 x 32k tokens, groups of eight, P = 256 / 128 / 64:
+//    305 / 308 / 343 us; 64 ragged sequences up to 8192 tokens, no groups, P = 64 / 32 / 16: 191 / 178 / 179 us.)
+// A plan from the actual lengths, as the ordinary kernels make for such calls, measured 317 to 390 us on the first of
+// these: parts of one wave end up to a third apart, whatever their lengths.
+int diff_splits(int cache_kind, int B, int heads, int pairs, int D, int64_t tiles, int sm) {
+  const int group = heads / pairs, per_sm = diff_items_per_sm(cache_kind, D, group);
+  const int64_t items = std::max<int64_t>(1, static_cast<int64_t>(B) * pairs), work = items * tiles;
+  const int64_t spread = static_cast<int64_t>(sm) * 4;
+  if (work < spread * 48) {
+    const int64_t S = std::min<int64_t>(spread / items, tiles / 2);
+    return static_cast<int>(std::min<int64_t>(S <= 32 ? S : S / 32 * 32, kMaxSplits));
   }
+  const int64_t wave = static_cast<int64_t>(sm) * std::max(4, per_sm - 1);
+  const int64_t longest = std::max<int64_t>(32, cache_kind == kCacheInt8 ? 16 * group : 8 * group);
+  if (work < wave * longest) return static_cast<int>(std::min<int64_t>(wave / items, kMaxSplits));
+  return static_cast<int>(std::min<int64_t>((tiles + longest - 1) / longest, kMaxSplits));
+}
+
+// Parts per sequence of a call; other shapes than the tiled ones have one item per query pair, see untiled_splits.
+int diff_parts(bool tiled, int cache_kind, int B, int heads, int pairs, int D, int64_t max_seq, int num_splits, int sm) {
+  const int64_t tiles = (max_seq + 15) / 16;
   int64_t S = num_splits;
-  if (S == 0) S = tiled ? choose_splits(B, pairs, max_seq, block_size, sm, false, wps) : untiled_splits(B, heads, heads, D, false, max_seq, sm);
-  t.S = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(S, tiles)));
-  t.need = std::max<int64_t>(diff_rows_bytes(static_cast<int64_t>(t.S) * B * 2 * heads, D), 16);
-  return t;
+  if (S == 0) S = tiled ? diff_splits(cache_kind, B, heads, pairs, D, tiles, sm) : untiled_splits(B, heads, heads, D, false, max_seq, sm);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(S, tiles)));
 }
 
 bool diff_tiled_shape(int D, int group, int block_size) {
@@ -1167,8 +1168,10 @@ int run_diff(const AttnCall& a, const DiffExtra& x) {
   const bool pair_rows = int8_cache && a.D == 64;
   const bool tiled = diff_tiled_shape(a.D, a.Hq / a.Hkv, a.block_size) && tma_friendly(a.kc, esz, a.kc_st, a.num_blocks) &&
                      tma_friendly(a.vc, esz, a.vc_st, a.num_blocks) && (!pair_rows || (a.kc_st[2] == 64 && a.vc_st[2] == 64));
-  const DiffPlan t = diff_plan(tiled, a.cache_kind, a.B, a.Hq, a.Hkv, a.D, max_seq, cap, a.block_size, a.num_splits, sm);
-  if (a.ws == nullptr || a.ws_bytes < t.need || (reinterpret_cast<uintptr_t>(a.ws) & 15u)) return INT8KV_E_WORKSPACE;
+  const int S = diff_parts(tiled, a.cache_kind, a.B, a.Hq, a.Hkv, a.D, max_seq, a.num_splits, sm);
+  if (a.ws == nullptr || (reinterpret_cast<uintptr_t>(a.ws) & 15u) ||
+      a.ws_bytes < diff_rows_bytes(static_cast<int64_t>(S) * a.B * 2 * a.Hq, a.D))
+    return INT8KV_E_WORKSPACE;
 
   DiffParams d;
   std::memset(&d, 0, sizeof(d));
@@ -1188,8 +1191,8 @@ int run_diff(const AttnCall& a, const DiffExtra& x) {
   p.sl = a.sl; p.sl_is_i64 = a.sl_is_i64;
   p.k_scale = a.k_scale; p.v_scale = a.v_scale;
   p.out = a.out; p.out_dtype = a.out_dtype;
-  p.num_splits = t.S;
-  p.per_longest = static_cast<int>(std::max<int64_t>(1, (tiles + t.S - 1) / t.S));
+  p.num_splits = S;
+  p.per_longest = static_cast<int>(std::max<int64_t>(1, (tiles + S - 1) / S));
   p.row_floats = partial_row_floats(2 * a.D);
   p.sm_scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(a.D)));
   p.status = a.status;
@@ -1198,15 +1201,6 @@ int run_diff(const AttnCall& a, const DiffExtra& x) {
     const int rc = launch_diff_generic(d, a.stream);
     return rc != INT8KV_OK ? rc : launch_diff_merge(d, a.stream);
   }
-  if (t.planned) {
-    p.plan_table = reinterpret_cast<int2*>(static_cast<char*>(a.ws) + t.table_off);
-    p.plan_grid_items = t.ps.max_items;
-    p.plan_slots = sm * diff_warps_per_sm(a.cache_kind, a.D, d.group);
-    p.plan_k_max = t.ps.k_max;
-    p.plan_min_part = t.ps.min_part;
-  } else if (t.S == 1) {
-    p.part = nullptr;  // whole sequences: the attention kernel writes `out`
-  }
   alignas(64) CUtensorMap tmK, tmV;
   auto map = [&](CUtensorMap* m, const void* base, const int64_t* st) {
     const int64_t pair_st[4] = {st[0], st[1], 2 * st[2], 1};
@@ -1214,8 +1208,8 @@ int run_diff(const AttnCall& a, const DiffExtra& x) {
                      : make_cache_map(m, base, esz, a.D, 2 * a.Hkv, a.num_blocks, a.block_size, st, 2);
   };
   if (!map(&tmK, a.kc, a.kc_st) || !map(&tmV, a.vc, a.vc_st)) return INT8KV_E_LAUNCH;
-  const int rc = launch_diff_tiled(d, tmK, tmV, sm, a.stream);
-  return rc != INT8KV_OK || t.S == 1 ? rc : launch_diff_merge(d, a.stream);
+  const int rc = launch_diff_tiled(d, tmK, tmV, a.stream);
+  return rc != INT8KV_OK ? rc : launch_diff_merge(d, a.stream);
 }
 
 }  // namespace
@@ -1228,17 +1222,12 @@ int64_t int8kv_diff_workspace_bytes(int batch, int num_heads, int num_kv_pairs, 
       max_seq_len < 0 || block_size <= 0 || num_splits < 0 || num_splits > kMaxSplits)
     return -1;
   const int sm = sm_count > 0 ? sm_count : 148;
-  int64_t need = 16;
+  int parts = 1;
   for (const int kind : {static_cast<int>(kCacheInt8), static_cast<int>(kCacheBf16)})
-    for (const bool tiled : {true, false}) {  // alignment and strides, which are not known here, decide between the two
-      if (tiled && !diff_tiled_shape(head_dim, num_heads / num_kv_pairs, block_size)) continue;
-      need = std::max(need, diff_plan(tiled, kind, batch, num_heads, num_kv_pairs, head_dim, max_seq_len, max_seq_len,
-                                      block_size, num_splits, sm).need);
-      // a table too wide for a device plan falls back to the fixed count
-      need = std::max(need, diff_plan(tiled, kind, batch, num_heads, num_kv_pairs, head_dim, max_seq_len,
-                                      int64_t(1) << 40, block_size, num_splits, sm).need);
-    }
-  return need;
+    for (const bool tiled : {true, false})  // alignment and strides, which are not known here, decide between the two
+      if (!tiled || diff_tiled_shape(head_dim, num_heads / num_kv_pairs, block_size))
+        parts = std::max(parts, diff_parts(tiled, kind, batch, num_heads, num_kv_pairs, head_dim, max_seq_len, num_splits, sm));
+  return diff_rows_bytes(static_cast<int64_t>(parts) * batch * 2 * num_heads, head_dim);
 }
 
 int int8kv_paged_diff_attn_int8(const void* query, int q_dtype, const int64_t q_strides[3], int batch, int num_heads,

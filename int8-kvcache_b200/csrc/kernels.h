@@ -180,9 +180,8 @@ struct DiffParams {
   float out_scale;
 };
 constexpr int kDiffMaxD = 256;
-constexpr int kDiffWarpsPerCta = 4;
-int diff_warps_per_sm(int cache_kind, int D, int group);  // resident warps per SM of the tiled kernel for a shape
-int launch_diff_tiled(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, int sm_count, cudaStream_t stream);
+int diff_items_per_sm(int cache_kind, int D, int group);  // resident items (CTAs) per SM of the tiled kernel for a shape
+int launch_diff_tiled(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t stream);
 int launch_diff_generic(const DiffParams& d, cudaStream_t stream);
 int launch_diff_merge(const DiffParams& d, cudaStream_t stream);
 

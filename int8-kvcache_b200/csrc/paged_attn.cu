@@ -150,12 +150,6 @@ __device__ __forceinline__ void chained_duty(const ChainedMerge& cm, int64_t ite
 // kDynScales = one scale per (token, head) read from scale caches beside the INT8 pages.
 constexpr int kPlain = 0, kFusedWrite = 1, kDynScales = 2;
 
-__device__ __forceinline__ float lds32f(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
-}
-
 // The fused step's write of the new token's row, once per (sequence, kv head): quantise the row exactly as the
 // cache-write kernel does, store it to the cache, and overwrite the row in the staged tile (TMA fetched the tile
 // before this store, so the stage still holds the old bytes).  Out of line on purpose: one warp in Hkv-th of the

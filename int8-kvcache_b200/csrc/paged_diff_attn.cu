@@ -7,8 +7,10 @@
 // What it has to read is the pair's K and V rows once, 4 D values per token, for both maps and all query pairs of the
 // group: HBM traffic bounds it, as it does ordinary decode attention.  Both maps therefore run in one pass over the
 // pages, each with its own running maximum and sum, and both are kept unnormalised until the end, because the
-// subtraction needs the two sums.  The parts of a split sequence leave one fp32 row [2 D values | log-sum-exp] per map
-// in the workspace (row 2h + map of the part); diff_merge_kernel joins the parts, subtracts, norms and writes.
+// subtraction needs the two sums.  Every part of a sequence leaves one fp32 row per map in the workspace (row 2h + map of
+// the part): [2 D sums of p v, before 1 / l and the V scales | m | l], with p = 2^(score - m) in log2 units and l the sum of
+// p; m = -inf marks an empty part, whose other values are not written.  diff_merge_kernel joins the parts, subtracts,
+// norms and writes.
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -19,7 +21,9 @@
 
 namespace int8kv {
 
-constexpr float kLn2 = 0.6931471805599453f;
+
+// The m of a partial row: a column of nothing but NaN has no reference (m = -inf) and must not pass for an empty part.
+__device__ __forceinline__ float part_ref(float m, float l) { return l != l ? l : m; }
 
 // ---------------------------------------------------------------------------------------------
 // Every shape: one warp per (sequence, query pair, split), lanes over the dims, four tokens per step, plain loads.
@@ -62,11 +66,10 @@ __global__ void __launch_bounds__(128) diff_generic_kernel(const DiffParams d) {
       q[m][s] = dd < D ? load_as_float(p.q, p.q_dtype, b * p.q_st[0] + (2 * h + m) * p.q_st[1] + dd * p.q_st[2]) : 0.f;
       acc[m][0][s] = acc[m][1][s] = 0.f;
     }
-  float ksc[2], vsc[2], mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float ksc[2], mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     ksc[m] = (p.k_scale ? fmaxf(__ldg(p.k_scale + 2 * pair + m), 1e-6f) : 1.f) * p.sm_scale_log2;
-    vsc[m] = p.v_scale ? fmaxf(__ldg(p.v_scale + 2 * pair + m), 1e-6f) : 1.f;
   }
   constexpr int kTok = 4;
   for (int64_t tok = tok_lo; tok < tok_hi; tok += kTok) {
@@ -149,22 +152,24 @@ __global__ void __launch_bounds__(128) diff_generic_kernel(const DiffParams d) {
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     float* out = p.part + (row + m) * p.row_floats;
-    const float inv = l[m] == 0.f ? 0.f : 1.f / l[m];  // a NaN sum stays one
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s) {
         const int dd = lane + kWarp * s;
-        if (dd < D) out[half * D + dd] = acc[m][half][s] * inv * vsc[half];
+        if (dd < D) out[half * D + dd] = acc[m][half][s];
       }
-    if (lane == 0) out[p.D] = l[m] == 0.f ? -INFINITY : (mx[m] + log2f(l[m])) * kLn2;
+    if (lane == 0) {
+      out[p.D] = part_ref(mx[m], l[m]);
+      out[p.D + 1] = l[m];
+    }
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // TMA-tiled kernels: D = 64 or 128, block size a multiple of 16, up to 8 query pairs per KV pair.
 //
-// One warp serves one (sequence, KV pair, split) with the ring of the ordinary tiled kernels; a stage holds a 16-token
+// One warp, a CTA of its own, serves one (sequence, KV pair, split) with the ring of the ordinary tiled kernels; a stage holds a 16-token
 // tile of both K heads and both halves of V, so every page byte is read once for both maps and the whole group.
 // Columns of the tensor-core tile (8 per block) are (map, query pair): up to 4 pairs share one block, columns 0-3 for
 // the first map and 4-7 for the second (NB = 1), larger groups use a block per map (NB = 2).  From the scores on the two
@@ -180,37 +185,61 @@ __device__ __forceinline__ int col_map(int nb, int c) { return NB == 1 ? c >> 2 
 template <int NB>
 __device__ __forceinline__ int col_pair(int c) { return NB == 1 ? c & 3 : c; }
 
-// Running softmax of the columns of one block: maximum and sum of columns 2t (index 0) and 2t+1.
+// Running softmax of the columns of one block: reference exponent and sum of columns 2t (index 0) and 2t+1.  The reference
+// m is a score that was the column's maximum when it was set; it follows the maximum only when that has moved more than
+// kSlack (in log2 units) above it, so probabilities reach up to 2^kSlack, which fp16, bf16 and the fp32 sums hold with the
+// same relative precision as values up to 1.  A step then needs no reduction across the token lanes, just a vote, and
+// the accumulators are rescaled a few times per part instead of in every other tile (measured on 32 x 32k tokens, groups
+// of 8: see the kernel).
+constexpr float kSlack = 8.f;
 struct ColStats {
   float m[2], l[2];
 };
 
-// One online-softmax step on a 16-token tile's C fragment v (log2 units, rows g / g+8, columns 2t / 2t+1): v becomes the
-// probabilities relative to the running maximum; returns whether the accumulators have to follow, by f[0], f[1].
-__device__ __forceinline__ bool softmax_step(ColStats& s, float (&v)[4], float (&f)[2]) {
-  float mx0 = fmaxf(v[0], v[2]), mx1 = fmaxf(v[1], v[3]);
-  mx0 = fmaxf(mx0, __shfl_xor_sync(kFull, mx0, 4));
-  mx1 = fmaxf(mx1, __shfl_xor_sync(kFull, mx1, 4));
-  mx0 = fmaxf(mx0, __shfl_xor_sync(kFull, mx0, 8));
-  mx1 = fmaxf(mx1, __shfl_xor_sync(kFull, mx1, 8));
-  mx0 = fmaxf(mx0, __shfl_xor_sync(kFull, mx0, 16));
-  mx1 = fmaxf(mx1, __shfl_xor_sync(kFull, mx1, 16));
-  const float mn0 = fmaxf(s.m[0], mx0), mn1 = fmaxf(s.m[1], mx1);
-  const bool moved = __any_sync(kFull, (mn0 != s.m[0]) || (mn1 != s.m[1]));
+// One online-softmax step over NV / 2 score rows per lane and NB column blocks at once (log2 units; v[nb][2k], v[nb][2k+1]
+// are columns 2t, 2t+1 of a row): v becomes the probabilities relative to the references; returns whether the
+// accumulators have to follow, by f[nb][0], f[nb][1].
+template <int NB, int NV>
+__device__ __forceinline__ bool softmax_step(ColStats (&s)[NB], float (&v)[NB][NV], float (&f)[NB][2]) {
+  float mx[NB][2];
+  bool high = false;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      mx[nb][e] = v[nb][e];
+#pragma unroll
+      for (int k = 2 + e; k < NV; k += 2) mx[nb][e] = fmaxf(mx[nb][e], v[nb][k]);
+      high = high || mx[nb][e] > s[nb].m[e] + kSlack;
+    }
+  const bool moved = __any_sync(kFull, high);
   if (moved) {
-    f[0] = exp2_fast(s.m[0] - mn0);
-    f[1] = exp2_fast(s.m[1] - mn1);
-    s.l[0] *= f[0];
-    s.l[1] *= f[1];
-    s.m[0] = mn0;
-    s.m[1] = mn1;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = mx[nb][e];
+        x = fmaxf(x, __shfl_xor_sync(kFull, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(kFull, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(kFull, x, 16));
+        x = fmaxf(x, s[nb].m[e]);
+        f[nb][e] = x == s[nb].m[e] ? 1.f : exp2_fast(s[nb].m[e] - x);  // equal also when nothing but -inf was seen
+        s[nb].l[e] *= f[nb][e];
+        s[nb].m[e] = x;
+      }
   }
-  v[0] = exp2_fast(v[0] - s.m[0]);
-  v[1] = exp2_fast(v[1] - s.m[1]);
-  v[2] = exp2_fast(v[2] - s.m[0]);
-  v[3] = exp2_fast(v[3] - s.m[1]);
-  s.l[0] += v[0] + v[2];
-  s.l[1] += v[1] + v[3];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[nb][k] = exp2_fast(v[nb][k] - s[nb].m[k & 1]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float sum = v[nb][e];
+#pragma unroll
+      for (int k = 2 + e; k < NV; k += 2) sum += v[nb][k];
+      s[nb].l[e] += sum;
+    }
+  }
   return moved;
 }
 
@@ -224,34 +253,96 @@ __device__ __forceinline__ void reduce_sums(ColStats& s) {
   }
 }
 
-__device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }  // a NaN sum stays one
-__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+// The ring of one item: tiles are issued and consumed in order, so stage, phase, block and tile-in-block are counters
+// instead of divisions of the tile number.
+template <int NST, int STAGE, int LOADS>
+struct DiffRing : TileRing<NST, STAGE, LOADS> {
+  int left;                 // tiles not issued yet
+  int in_stage, in_idx, in_sub;  // next tile to issue: stage, block relative to lb0, tile inside the block
+  int out_stage;            // next tile to consume
+  uint32_t out_phase;
 
-// Result of an empty tile range.
-__device__ __forceinline__ void diff_write_empty(const DiffParams& d, const ItemCoord& it, int lane, float* prow) {
-  const AttnParams& p = d.a;
-  if (prow != nullptr) {
-    if (lane < p.G) prow[lane * p.row_floats + p.D] = -INFINITY;
-    return;
+  __device__ __forceinline__ void start(const ItemCoord& it) {
+    left = it.t1 - it.t0;
+    in_stage = in_idx = out_stage = 0;
+    out_phase = 0u;
+    in_sub = it.t0 - this->lb0 * this->tpb;
   }
-  for (int hg = 0; hg < d.group; ++hg) {
-    const int64_t base = it.b * p.o_st[0] + (it.h * d.group + hg) * p.o_st[1];
-    for (int i = lane; i < p.D; i += kWarp) store_from_float(p.out, p.out_dtype, base + i * p.o_st[2], 0.f);
+  __device__ __forceinline__ void issue_next() {  // called by all lanes
+    if (left <= 0) return;
+    --left;
+    const int win = in_idx >> 5;
+    if (win != this->cur_win) {
+      this->bt_cur = this->bt_next;
+      this->cur_win = win;
+      this->bt_next = this->load_window(win + 1);
+    }
+    const int blk = __shfl_sync(kFull, this->bt_cur, in_idx & 31);
+    if (this->lane == 0) {
+      const uint32_t bar = this->bar0 + 8 * in_stage, dst = this->stage0 + in_stage * STAGE;
+      mbar_expect_tx(bar, STAGE);
+#pragma unroll
+      for (int x = 0; x < LOADS; ++x)
+        tma_load_4d(dst + x * this->PIECE, this->tmK, bar, x * 128, in_sub * kTile, this->head, blk, this->kv_policy);
+#pragma unroll
+      for (int x = 0; x < LOADS; ++x)
+        tma_load_4d(dst + (LOADS + x) * this->PIECE, this->tmV, bar, x * 128, in_sub * kTile, this->head, blk, this->kv_policy);
+    }
+    in_stage = in_stage + 1 == NST ? 0 : in_stage + 1;
+    if (++in_sub == this->tpb) {
+      in_sub = 0;
+      ++in_idx;
+    }
   }
+  __device__ __forceinline__ void fill() {
+#pragma unroll 1
+    for (int i = 0; i < NST; ++i) issue_next();
+  }
+  // Stage of tile u of this trip (u = 0, 1).
+  __device__ __forceinline__ int stage_index(int u) const {
+    const int x = out_stage + u;
+    return x >= NST ? x - NST : x;
+  }
+  __device__ __forceinline__ uint32_t stage_addr(int u) const { return this->stage0 + stage_index(u) * STAGE; }
+  // Wait for tile u of this trip; false if the bounded wait ran out on any lane.
+  __device__ __forceinline__ bool wait_tile(int u, uint32_t limit = kWaitSpinLimit) const {
+    const int x = out_stage + u;
+    const bool ok = mbar_wait_bounded(this->bar0 + 8 * stage_index(u), x >= NST ? out_phase ^ 1u : out_phase, limit);
+    return __all_sync(kFull, ok);
+  }
+  // The trip's `count` tiles are consumed: their stages are refilled.
+  __device__ __forceinline__ void advance(int count) {
+    out_stage += count;
+    if (out_stage >= NST) {
+      out_stage -= NST;
+      out_phase ^= 1u;
+    }
+    __syncwarp();  // every lane has read the stages
+    for (int k = 0; k < count; ++k) issue_next();
+  }
+  // A wait ran out: report it, and wait, again with a limit, for the `flying` tiles that were issued and not consumed.
+  __device__ __forceinline__ void give_up(const AttnParams& p, int flying) {
+    if (this->lane == 0 && p.status != nullptr) atomicOr(p.status, INT8KV_DEV_WAIT_TIMEOUT);
+    for (int u = 0; u < flying; ++u) {
+      wait_tile(0, 1u << 12);
+      if (++out_stage == NST) {
+        out_stage = 0;
+        out_phase ^= 1u;
+      }
+    }
+  }
+};
+
+// Whether the queries are rows that 16-byte loads can read: then nothing is staged through the idle ring.
+__device__ __forceinline__ bool direct_queries(const AttnParams& p) {
+  const int64_t unit = p.q_dtype == INT8KV_FP32 ? 4 : 8;  // elements per 16 bytes
+  return p.q_st[2] == 1 && (reinterpret_cast<uintptr_t>(p.q) & 15u) == 0 && p.q_st[0] % unit == 0 && p.q_st[1] % unit == 0;
 }
 
-// The work item of a warp: coordinates, tile range, first partial row (null: the result goes to `out`), and the ring
-// ready to issue.  Returns false when the warp has nothing (more) to do.
-template <bool PLANNED, typename Ring>
-__device__ __forceinline__ bool diff_begin(const DiffParams& d, Ring& ring, ItemCoord& it, float*& prow, int64_t item,
-                                           int heads_per_box, int lane) {
+// The work item of a one-warp CTA, first half: coordinates; everything up to the first global read.
+template <typename Ring>
+__device__ __forceinline__ void diff_item(const DiffParams& d, Ring& ring, ItemCoord& it, int lane, int heads_per_box) {
   const AttnParams& p = d.a;
-  int64_t row0;
-  if constexpr (PLANNED) {
-    if (item >= p.plan_grid_items) return false;
-  } else {
-    if (!item_coords(p, item, it)) return false;
-  }
   ring.bt_is_i64 = p.bt_is_i64;
   ring.bt_stride = p.bt_st[1];
   ring.bt_limit = p.bt_width;
@@ -263,36 +354,100 @@ __device__ __forceinline__ bool diff_begin(const DiffParams& d, Ring& ring, Item
   ring.init_barriers(lane);
   grid_dependency_wait();  // from here on global memory is read
   grid_launch_dependents();
-  if constexpr (PLANNED) {
-    PlanNote note;
-    const bool live = plan_in_warp(p, item, lane, it, row0, note);
-    plan_commit(p, note, lane);
-    if (!live) return false;
-  }
+  item_coords(p, blockIdx.x, it);  // the grid is exactly the items
   ring.bt_row = reinterpret_cast<const char*>(p.bt) + it.b * p.bt_st[0] * (p.bt_is_i64 ? 8 : 4);
   ring.head = it.h * heads_per_box;
-  if constexpr (PLANNED) {
-    ring.prefetch_tables(it.t0 / p.tiles_per_block);
-  } else {
-    ring.prefetch_tables(guessed_first_block(p, it.c));
-    item_range(p, it);
-    row0 = arithmetic_row0(p, it);
-  }
-  prow = result_row(p, it, row0);
-  if (it.t0 >= it.t1) {
-    diff_write_empty(d, it, lane, prow);
+}
+
+// Second half: tile range, the first of the item's 2 * group partial rows, and the first tiles under way (unless `hold`).
+// Returns false when the part is empty.
+template <typename Ring>
+__device__ __forceinline__ bool diff_range(const DiffParams& d, Ring& ring, ItemCoord& it, float*& prow, int lane, bool hold) {
+  const AttnParams& p = d.a;
+  ring.prefetch_tables(guessed_first_block(p, it.c));
+  item_range(p, it);
+  prow = p.part + arithmetic_row0(p, it) * p.row_floats;
+  if (it.t0 >= it.t1) {  // rows that the join skips
+    if (lane < p.G) prow[lane * p.row_floats + p.D] = -INFINITY;
     return false;
   }
   ring.set_range(it.t0, p.tiles_per_block);
+  ring.start(it);
+  if (!hold) ring.fill();
   return true;
 }
 
-// A wait ran out at tile i of n: report it, and wait (again with a limit) for the loads that are still in flight.
-template <int NST, typename Ring>
-__device__ __forceinline__ void diff_timed_out(const AttnParams& p, const Ring& ring, int i, int n, int lane) {
-  if (lane == 0 && p.status != nullptr) atomicOr(p.status, INT8KV_DEV_WAIT_TIMEOUT);
-  const int issued = (i + NST < n) ? i + NST : n;
-  for (int j = i; j < issued; ++j) ring.wait(j, 1u << 12);
+// 16 bytes of a query, requested at this place in the program (the values are used much later).
+__device__ __forceinline__ uint4 ldg_early(const void* ptr) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
+  return v;
+}
+
+// Two 16-bit floats -> floats.
+__device__ __forceinline__ float2 unpack16(uint32_t w, int dtype) {
+  if (dtype == INT8KV_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Queries of a column as two INT8 limbs, q ~= q_mul * (256 hi + lo) with |256 hi + lo| <= 32000: 16-bit fixed point per
+// head, so that the K bytes go to the INT8 tensor cores as they lie in the cache.  The 1.5 * 2^23 addition of the
+// FMA rounds and leaves the integer in the low mantissa bits.  `abits`: bits of the largest magnitude of this lane's
+// elements.  A NaN or infinity in a head makes q_mul NaN, and with it the
+// head's output.
+struct QueryScale {
+  float inv, mul;
+};
+template <int LANES>  // lanes that share a head: the column's four, or two (D = 64 with a block per map)
+__device__ __forceinline__ QueryScale query_scale(uint32_t abits) {
+  abits = max(abits, __shfl_xor_sync(kFull, abits, 1));
+  if (LANES == 4) abits = max(abits, __shfl_xor_sync(kFull, abits, 2));
+  const float amax = __uint_as_float(abits);
+  QueryScale s;
+  const bool live = amax > 1e-20f;
+  s.inv = live ? __fdividef(32000.f, amax) : 0.f;
+  s.mul = live ? __fdividef(1.f, s.inv) : 0.f;
+  if (abits >= 0x7f800000u) s.mul = __uint_as_float(0x7fffffffu);
+  return s;
+}
+__device__ __forceinline__ void query_limbs(float a, float b, float c, float e, float inv, uint32_t& lo, uint32_t& hi) {
+  const float t0 = fmaf(a, inv, kRoundMagic), t1 = fmaf(b, inv, kRoundMagic), t2 = fmaf(c, inv, kRoundMagic), t3 = fmaf(e, inv, kRoundMagic);
+  lo = prmt(prmt(__float_as_uint(t0), __float_as_uint(t1), 0x0040u), prmt(__float_as_uint(t2), __float_as_uint(t3), 0x0040u), 0x5410u);
+  // the second byte of v + 128 is round(v / 256): adding 128 to the float is exact
+  hi = prmt(prmt(__float_as_uint(t0 + 128.f), __float_as_uint(t1 + 128.f), 0x0051u),
+            prmt(__float_as_uint(t2 + 128.f), __float_as_uint(t3 + 128.f), 0x0051u), 0x5410u);
+}
+
+// The item's partial rows go through shared memory (the ring's stages, free by then) and leave as whole lines: written from
+// the fragments (16 bytes per lane, 64 bytes apart) they would reach the workspace as 1024 half-written sectors per
+// warp, 2.2 us at the end of every item.  Lane t's rows lie in slots t, t + 4, ..., a row (a multiple of 128 bytes plus
+// 16) apart, so that a warp's 16-byte stores spread over all banks.
+template <int NB>
+__device__ __forceinline__ int row_slot(int nb, int e, int t) { return t + 4 * (e + 2 * nb); }
+
+template <int NB, int VALUES>
+__device__ __forceinline__ void store_rows(float* prow, uint32_t slots, int group, int lane) {
+  constexpr int kRow = VALUES + 4;  // floats
+  __syncwarp();
+#pragma unroll 4
+  for (int slot = 0; slot < 8 * NB; ++slot) {
+    const int t = slot & 3, e = (slot >> 2) & 1, nb = slot >> 3;
+    const int hg = col_pair<NB>(2 * t + e), m = col_map<NB>(nb, 2 * t + e);
+    if (hg >= group) continue;
+    float* dst = prow + (2 * hg + m) * kRow;
+#pragma unroll
+    for (int i = 0; i < VALUES; i += 128) {
+      const uint4 x = lds128(slots + (slot * kRow + i + 4 * lane) * 4);
+      *reinterpret_cast<uint4*>(dst + i + 4 * lane) = x;
+    }
+    if (lane == 0) *reinterpret_cast<uint4*>(dst + VALUES) = lds128(slots + (slot * kRow + VALUES) * 4);
+  }
+}
+__device__ __forceinline__ void sts128(uint32_t addr, float a, float b, float c, float e) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(e) : "memory");
+}
+__device__ __forceinline__ void sts32(uint32_t addr, float a) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(a) : "memory");
 }
 
 // Eight dims x 16 tokens of V^T per step, INT8 -> fp16 on the way (see pv_tile), times P^T of NB column blocks.
@@ -317,104 +472,163 @@ __device__ __forceinline__ void pv_blocks(float (&acc)[NB][8][4], const uint4 (&
   }
 }
 
-// Resident warps per SM and ring depth: 192 KB of ring per SM in every variant (the bytes in flight that keep HBM busy);
-// a stage is 8 KB for D = 128 and 4 KB for D = 64.  The accumulators, 32 floats per lane and (column block, 128 values
-// of V), set how many warps the register file carries.
+// Scores of one 16-token tile against every column, as integers: s[nb] = 256 (K . Qhi) + (K . Qlo) on the C fragment.
+// The limbs' and blocks' chains of MMAs run side by side.
+template <int DK, int NB>
+__device__ __forceinline__ void diff_scores(int (&s)[NB][4], uint32_t kb, const uint32_t (&koff)[4], const uint32_t (&qh)[NB][8],
+                                            const uint32_t (&ql)[NB][8], int t) {
+  constexpr int KT = DK / 64;                 // K tiles: the two heads' (D = 128), or one of both (D = 64)
+  constexpr int CH = NB > KT ? NB : KT;       // chains: block nb against its map's tile; NB = 1, D = 128: both tiles
+  uint32_t ka[KT][8], kc[KT][8];
+#pragma unroll
+  for (int k = 0; k < KT; ++k) {
+    const uint4 a0 = lds128(kb + k * 2048 + koff[0]), a1 = lds128(kb + k * 2048 + koff[1]);
+    const uint4 c0 = lds128(kb + k * 2048 + koff[2]), c1 = lds128(kb + k * 2048 + koff[3]);
+    ka[k][0] = a0.x; ka[k][1] = a0.y; ka[k][2] = a0.z; ka[k][3] = a0.w; ka[k][4] = a1.x; ka[k][5] = a1.y; ka[k][6] = a1.z; ka[k][7] = a1.w;
+    kc[k][0] = c0.x; kc[k][1] = c0.y; kc[k][2] = c0.z; kc[k][3] = c0.w; kc[k][4] = c1.x; kc[k][5] = c1.y; kc[k][6] = c1.z; kc[k][7] = c1.w;
+  }
+  int lo[CH][4], hi[CH][4];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lo[c][r] = hi[c][r] = 0;
+#pragma unroll
+  for (int st = 0; st < 4; ++st)
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int k = KT == 1 ? 0 : c, nb = NB == 1 ? 0 : c;
+      mma_s8(lo[c], ka[k][2 * st], kc[k][2 * st], ka[k][2 * st + 1], kc[k][2 * st + 1], ql[nb][2 * st], ql[nb][2 * st + 1]);
+      mma_s8(hi[c], ka[k][2 * st], kc[k][2 * st], ka[k][2 * st + 1], kc[k][2 * st + 1], qh[nb][2 * st], qh[nb][2 * st + 1]);
+    }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (CH > NB) s[nb][r] = t < 2 ? (hi[0][r] << 8) + lo[0][r] : (hi[CH - 1][r] << 8) + lo[CH - 1][r];  // own map's tile
+      else s[nb][r] = (hi[nb][r] << 8) + lo[nb][r];
+    }
+}
+
+// Items resident per SM and ring depth: 192 KB of ring per SM (the bytes in flight that keep HBM busy); a stage is 8 KB
+// for D = 128 and 4 KB for D = 64.  kTrip tiles are consumed per trip: with 4 KB tiles two, for which one softmax step
+// serves both.  The accumulators, 32 floats per lane and (column block, 128 values of V), set how many warps the register
+// file carries.
 template <int DK, int NB>
 struct DiffInt8Shape {
   static constexpr int kHalves = DK / 64;
   static constexpr int kStage = kHalves * 4096;
-  static constexpr int kWarpsPerSm = kHalves * NB == 1 ? 12 : 8;
-  static constexpr int kStages = 192 * 1024 / (kWarpsPerSm * kStage);
+  static constexpr int kTrip = DK == 128 ? 1 : 2;
+  static constexpr int kPerSm = DK == 64 && NB == 1 ? 12 : 8;
+  static constexpr int kStages = 192 * 1024 / (kPerSm * kStage);
+  static constexpr int kSmem = kStages * (kStage + 8) + 1024;
 };
 
-template <int DK, int NB, bool PLANNED>
-__global__ void __launch_bounds__(kDiffWarpsPerCta * kWarp, DiffInt8Shape<DK, NB>::kWarpsPerSm / kDiffWarpsPerCta)
+template <int DK, int NB>
+__global__ void __launch_bounds__(kWarp, DiffInt8Shape<DK, NB>::kPerSm)
 diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ DiffParams d) {
   using Shape = DiffInt8Shape<DK, NB>;
-  constexpr int HV = Shape::kHalves, NST = Shape::kStages, STAGE = Shape::kStage;
+  constexpr int NST = Shape::kStages, STAGE = Shape::kStage, TRIP = Shape::kTrip, HV = Shape::kHalves;
+  constexpr int QB = DK == 64 ? 1 : NB;  // rows of 32 query values per lane (D = 64: a lane's half row is one map's)
   extern __shared__ uint8_t smem_raw[];
   const AttnParams& p = d.a;
-  const int wpc = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x, g = lane >> 2, t = lane & 3;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  TileRing<NST, STAGE, 1> ring;
-  ring.stage0 = smem_base + warp * (NST * STAGE);
-  ring.bar0 = smem_base + wpc * NST * STAGE + warp * (NST * 8);
+  DiffRing<NST, STAGE, 1> ring;
+  ring.stage0 = smem_base;
+  ring.bar0 = smem_base + NST * STAGE;
   ring.tmK = &tmK;
   ring.tmV = &tmV;
   ItemCoord it;
   float* prow;
-  if (!diff_begin<PLANNED>(d, ring, it, prow, static_cast<int64_t>(blockIdx.x) * wpc + warp, HV, lane)) return;
+  diff_item(d, ring, it, lane, HV);
 
-  const float ks0 = __ldg(p.k_scale + 2 * it.h), ks1 = __ldg(p.k_scale + 2 * it.h + 1);
-  const float vs0 = __ldg(p.v_scale + 2 * it.h), vs1 = __ldg(p.v_scale + 2 * it.h + 1);
-  // The queries are requested first (a strided or unaligned one is staged through the idle ring), then the tiles; the
-  // queries' arithmetic runs while the tiles are in flight.  Lane (g, t) holds column g's dims [32t, 32t+32) of the
-  // 128-value tile row.
-  float qv[NB][32];
-  auto load_query = [&](int m, int hg, int dim, float (&x)[32]) {
-    load32_as_float(p.q, p.q_dtype, it.b * p.q_st[0] + (2 * (it.h * d.group + hg) + m) * p.q_st[1] + dim * p.q_st[2],
-                    p.q_st[2], x, ring.stage0, lane);
-  };
-  if constexpr (DK == 64 && NB == 2) {  // the lane's half of the row belongs to one map, that is to one block
-    float x[32];
-    const bool live = g < d.group;
-    if (live) load_query(t >> 1, g, 32 * (t & 1), x);
+  // Lane (g, t) holds column g's dims [32t, 32t+32) of the 128-value tile row.  Rows of 16-bit values that 16-byte loads
+  // can read (the usual case) are requested ahead of lengths, tables and tiles, and converted while the tiles are in
+  // flight; any other layout is staged through the ring's first stage, ahead of the tiles.
+  const bool direct = direct_queries(p), raw16 = direct && p.q_dtype != INT8KV_FP32;
+  int64_t q_at[QB];
+  bool q_live[QB];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      qv[0][i] = live && t < 2 ? x[i] : 0.f;
-      qv[1][i] = live && t >= 2 ? x[i] : 0.f;
+  for (int k = 0; k < QB; ++k) {
+    const int m = DK == 64 ? t >> 1 : col_map<NB>(k, g), hg = col_pair<NB>(g);
+    q_live[k] = hg < d.group && (DK == 128 || NB == 2 || m == col_map<NB>(0, g));
+    q_at[k] = it.b * p.q_st[0] + (2 * (it.h * d.group + hg) + m) * p.q_st[1] + (DK == 128 ? 32 * t : 32 * (t & 1)) * p.q_st[2];
+  }
+  uint4 raw[QB][4];
+#pragma unroll
+  for (int k = 0; k < QB; ++k)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      raw[k][w] = make_uint4(0u, 0u, 0u, 0u);
+      if (raw16 && q_live[k]) raw[k][w] = ldg_early(reinterpret_cast<const uint16_t*>(p.q) + q_at[k] + 8 * w);
+    }
+  const float ks0 = __ldg(p.k_scale + 2 * it.h), ks1 = __ldg(p.k_scale + 2 * it.h + 1);
+  if (!diff_range(d, ring, it, prow, lane, !direct)) return;
+  const int n = it.t1 - it.t0;
+
+  uint32_t qh[NB][8], ql[NB][8];
+  float q_mul[QB];
+  if (raw16) {
+#pragma unroll
+    for (int k = 0; k < QB; ++k) {
+      uint32_t top = 0u;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(&raw[k][i >> 2])[i & 3] & 0x7fff7fffu);
+      top = max(top & 0xffffu, top >> 16);  // magnitudes of 16-bit floats order like their bits
+      const float2 amax = unpack16(top, p.q_dtype);
+      const QueryScale sc = query_scale<DK == 64 && NB == 2 ? 2 : 4>(__float_as_uint(amax.x));
+      q_mul[k] = sc.mul;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4& r = raw[k][i >> 1];
+        const float2 x = unpack16(i & 1 ? r.z : r.x, p.q_dtype), y = unpack16(i & 1 ? r.w : r.y, p.q_dtype);
+        query_limbs(x.x, x.y, y.x, y.y, sc.inv, ql[k][i], qh[k][i]);
+      }
     }
   } else {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int m = col_map<NB>(nb, g), hg = col_pair<NB>(g);
-      if (hg < d.group && (DK == 128 || (t >> 1) == m)) {
-        load_query(m, hg, DK == 128 ? 32 * t : 32 * (t & 1), qv[nb]);
+    for (int k = 0; k < QB; ++k) {
+      float x[32];
+      if (q_live[k]) {
+        load32_as_float(p.q, p.q_dtype, q_at[k], p.q_st[2], x, ring.stage0, lane);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) qv[nb][i] = 0.f;
+        for (int i = 0; i < 32; ++i) x[i] = 0.f;
       }
+      uint32_t abits = 0u;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) abits = max(abits, __float_as_uint(x[i]) & 0x7fffffffu);
+      const QueryScale sc = query_scale<DK == 64 && NB == 2 ? 2 : 4>(abits);
+      q_mul[k] = sc.mul;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) query_limbs(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], sc.inv, ql[k][i], qh[k][i]);
+    }
+    if (!direct) {
+      fence_proxy_async_smem();  // the queries were staged by the lanes; the first tile is written by the TMA unit
+      __syncwarp();
+      ring.fill();
     }
   }
-  fence_proxy_async_smem();  // a staged query was written by the lanes; the first tile is written by the TMA unit
-  __syncwarp();
-  const int n = it.t1 - it.t0;
-  const int pre = n < NST ? n : NST;
-  for (int i = 0; i < pre; ++i) ring.issue(i);
-
-  // Queries as two INT8 limbs, q ~= q_mul * (256 hi + lo) with |256 hi + lo| <= 32000: 16-bit fixed point per head, so
-  // that the K bytes go to the INT8 tensor cores as they lie in the cache.  A NaN or infinity in a head makes its
-  // multiplier NaN, and with it the head's output.
-  uint32_t qh[NB][8], ql[NB][8];
+  if constexpr (DK == 64 && NB == 2) {  // the row belongs to one map, that is to one block; zero in the other
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ql[1][i] = t >= 2 ? ql[0][i] : 0u;
+      qh[1][i] = t >= 2 ? qh[0][i] : 0u;
+      ql[0][i] = t < 2 ? ql[0][i] : 0u;
+      qh[0][i] = t < 2 ? qh[0][i] : 0u;
+    }
+  }
+  // score multipliers of columns 2t and 2t+1, which belong to the same map; D = 64, NB = 2: lanes 0, 1 of a column hold
+  // the first map's scale, lanes 2, 3 the second's
   float sc[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    uint32_t abits = 0u;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) abits = max(abits, __float_as_uint(qv[nb][i]) & 0x7fffffffu);
-    abits = max(abits, __shfl_xor_sync(kFull, abits, 1));
-    abits = max(abits, __shfl_xor_sync(kFull, abits, 2));
-    const float amax = __uint_as_float(abits);
-    const bool live_q = amax > 1e-20f;
-    const float inv = live_q ? __fdividef(32000.f, amax) : 0.f;
-    float q_mul = live_q ? __fdividef(1.f, inv) : 0.f;
-    if (abits >= 0x7f800000u) q_mul = __uint_as_float(0x7fffffffu);
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      uint32_t v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        v[k] = static_cast<uint32_t>(__float_as_int(fmaf(qv[nb][4 * w + k], inv, kRoundMagic)) - kRoundMagicBits);
-      ql[nb][w] = prmt(prmt(v[0], v[1], 0x0040u), prmt(v[2], v[3], 0x0040u), 0x5410u);
-      qh[nb][w] = prmt(prmt(v[0] + 128u, v[1] + 128u, 0x0051u), prmt(v[2] + 128u, v[3] + 128u, 0x0051u), 0x5410u);
-    }
-    // score multipliers of columns 2t and 2t+1, which belong to the same map
+    const float mul = q_mul[QB == 1 ? 0 : nb];
+    const int holder = DK == 64 && NB == 2 ? 2 * nb : 0;
     const float kmul = fmaxf(col_map<NB>(nb, 2 * t) ? ks1 : ks0, 1e-6f) * p.sm_scale_log2;
-    sc[nb][0] = kmul * __shfl_sync(kFull, q_mul, (2 * t) * 4);
-    sc[nb][1] = kmul * __shfl_sync(kFull, q_mul, (2 * t + 1) * 4);
+    sc[nb][0] = kmul * __shfl_sync(kFull, mul, (2 * t) * 4 + holder);
+    sc[nb][1] = kmul * __shfl_sync(kFull, mul, (2 * t + 1) * 4 + holder);
   }
 
   const uint32_t koff[4] = {swz128(g, 2 * t), swz128(g, 2 * t + 1), swz128(g + 8, 2 * t), swz128(g + 8, 2 * t + 1)};
@@ -431,134 +645,78 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
       for (int j = 0; j < 8; ++j) acc[h][nb][j][0] = acc[h][nb][j][1] = acc[h][nb][j][2] = acc[h][nb][j][3] = 0.f;
   }
 
-  for (int i = 0; i < n; ++i) {
-    if (!ring.wait(i)) {
-      diff_timed_out<NST>(p, ring, i, n, lane);
+  // When the range holds an odd number of tiles the last trip of two has one all masked tile; its stage holds finite
+  // integers, stale or fresh, that meet p = 0.
+  for (int i = 0; i < n; i += TRIP) {
+    bool ok = ring.wait_tile(0);
+    if (TRIP == 2 && ok && i + 1 < n) ok = ring.wait_tile(1);
+    if (!ok) {
+      ring.give_up(p, min(NST, n - i));
       return;
     }
-    const uint32_t kb = ring.stage(i), vb = kb + STAGE / 2;
-    int raw[NB][4];
-    if constexpr (DK == 128 && NB == 1) {  // both K tiles against all columns; each column keeps its own map's score
-      int second[4];
-      qk_tile(raw[0], kb, koff, qh[0], ql[0], true);
-      qk_tile(second, kb + 2048, koff, qh[0], ql[0], true);
+    float v[NB][4 * TRIP], f[NB][2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) raw[0][r] = t < 2 ? raw[0][r] : second[r];
-    } else {
+    for (int u = 0; u < TRIP; ++u) {
+      int raw[NB][4];
+      diff_scores<DK, NB>(raw, ring.stage_addr(u), koff, qh, ql, t);
+      const int tok = (it.t0 + i + u) * kTile + g;
+      const bool in_lo = i + u < n && tok < it.seq_len, in_hi = i + u < n && tok + 8 < it.seq_len;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) qk_tile(raw[nb], DK == 128 ? kb + nb * 2048 : kb, koff, qh[nb], ql[nb], true);
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          v[nb][4 * u + r] = (r < 2 ? in_lo : in_hi) ? static_cast<float>(raw[nb][r]) * sc[nb][r & 1] : -INFINITY;
     }
-    uint4 vx[HV][4];
+    if (softmax_step<NB, 4 * TRIP>(st, v, f)) {
+#pragma unroll
+      for (int h = 0; h < HV; ++h)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            acc[h][nb][j][0] *= f[nb][0]; acc[h][nb][j][1] *= f[nb][1]; acc[h][nb][j][2] *= f[nb][0]; acc[h][nb][j][3] *= f[nb][1];
+          }
+    }
+    // P^T as B operands, rounded to fp16 (the sum keeps the unrounded values)
+    uint32_t pb[TRIP][NB][2];
+#pragma unroll
+    for (int u = 0; u < TRIP; ++u)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        pb[u][nb][0] = movmatrix_trans(pack_half2(v[nb][4 * u], v[nb][4 * u + 1]));
+        pb[u][nb][1] = movmatrix_trans(pack_half2(v[nb][4 * u + 2], v[nb][4 * u + 3]));
+      }
 #pragma unroll
     for (int h = 0; h < HV; ++h)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) vx[h][r] = lds128(vb + h * 2048 + voff[r]);
-
-    const int tok0 = (it.t0 + i) * kTile + g;
-    uint32_t pb[NB][2];
+      for (int u = 0; u < TRIP; ++u) {
+        uint4 vx[4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float v[4], f[2];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(raw[nb][r]) * sc[nb][r & 1];
-      if (tok0 >= it.seq_len) v[0] = v[1] = -INFINITY;
-      if (tok0 + 8 >= it.seq_len) v[2] = v[3] = -INFINITY;
-      if (softmax_step(st[nb], v, f)) {
-#pragma unroll
-        for (int h = 0; h < HV; ++h)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            acc[h][nb][j][0] *= f[0]; acc[h][nb][j][1] *= f[1]; acc[h][nb][j][2] *= f[0]; acc[h][nb][j][3] *= f[1];
-          }
+        for (int r = 0; r < 4; ++r) vx[r] = lds128(ring.stage_addr(u) + STAGE / 2 + h * 2048 + voff[r]);
+        pv_blocks<NB>(acc[h], vx, pb[u]);
       }
-      // P^T as B operands, rounded to fp16 (the sum keeps the unrounded values)
-      pb[nb][0] = movmatrix_trans(pack_half2(v[0], v[1]));
-      pb[nb][1] = movmatrix_trans(pack_half2(v[2], v[3]));
-    }
-#pragma unroll
-    for (int h = 0; h < HV; ++h) pv_blocks<NB>(acc[h], vx[h], pb);
-
-    __syncwarp();  // every lane has consumed the stage before lane 0 refills it
-    if (i + NST < n) ring.issue(i + NST);
+    ring.advance(TRIP);
   }
 
-  // ---- epilogue: lane (g, t) holds dims 128 h + 16 g .. + 15 of columns 2t and 2t+1 ----------------------
-  const float v0 = fmaxf(vs0, 1e-6f), v1 = fmaxf(vs1, 1e-6f);
+  // ---- epilogue: lane (g, t) holds dims 128 h + 16 g .. + 15 of columns 2t and 2t+1 ---------------------------
+  constexpr int kRow = (2 * DK + 4) * 4;  // bytes of a partial row
+  static_assert(16 * kRow <= NST * STAGE, "the rows of a group fit the ring");
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     reduce_sums(st[nb]);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float inv = inv_sum(st[nb].l[e]);
+    for (int e = 0; e < 2; ++e) {  // (columns without a query pair write slots that are not copied out)
+      const uint32_t row = ring.stage0 + row_slot<NB>(nb, e, t) * kRow;
 #pragma unroll
-      for (int h = 0; h < HV; ++h) {
-        const float f = inv * (DK == 128 ? (h ? v1 : v0) : (g >= 4 ? v1 : v0));
+      for (int h = 0; h < HV; ++h)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          acc[h][nb][j][e] *= f;
-          acc[h][nb][j][e + 2] *= f;
-        }
-      }
+        for (int k = 0; k < 4; ++k)
+          sts128(row + (128 * h + 16 * g + 4 * k) * 4, acc[h][nb][2 * k][e], acc[h][nb][2 * k][e + 2], acc[h][nb][2 * k + 1][e],
+                 acc[h][nb][2 * k + 1][e + 2]);
+      if (g == 0) sts128(row + 2 * DK * 4, part_ref(st[nb].m[e], st[nb].l[e]), st[nb].l[e], 0.f, 0.f);
     }
   }
-  if (prow != nullptr) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int hg = col_pair<NB>(2 * t + e), m = col_map<NB>(nb, 2 * t + e);
-        if (hg >= d.group) continue;
-        float* row = prow + (2 * hg + m) * p.row_floats;
-#pragma unroll
-        for (int h = 0; h < HV; ++h) {
-          float4* dst = reinterpret_cast<float4*>(row + 128 * h + 16 * g);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            dst[k] = make_float4(acc[h][nb][2 * k][e], acc[h][nb][2 * k][e + 2], acc[h][nb][2 * k + 1][e], acc[h][nb][2 * k + 1][e + 2]);
-        }
-        if (g == 0) row[p.D] = lse_of(st[nb].m[e], st[nb].l[e]);
-      }
-    return;
-  }
-  // a sequence in one part: subtract, norm and write here.  The second map's column sits two lanes on (NB = 1) or in
-  // the second block.
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int hg = col_pair<NB>(2 * t + e);
-    const bool mine = hg < d.group && (NB == 2 || t < 2);
-    const int head = it.h * d.group + (mine ? hg : 0);
-    const float lam = load_as_float(d.lam, d.lam_dtype, head * d.lam_st);
-    float o[HV][16], sq = 0.f;
-#pragma unroll
-    for (int h = 0; h < HV; ++h)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float a = acc[h][0][k >> 1][e + 2 * (k & 1)];
-        const float b = NB == 2 ? acc[h][NB - 1][k >> 1][e + 2 * (k & 1)] : __shfl_xor_sync(kFull, a, 2);
-        o[h][k] = a - lam * b;
-        sq = fmaf(o[h][k], o[h][k], sq);
-      }
-    float f = d.out_scale;
-    if (d.norm_w != nullptr) {
-      sq += __shfl_xor_sync(kFull, sq, 4);
-      sq += __shfl_xor_sync(kFull, sq, 8);
-      sq += __shfl_xor_sync(kFull, sq, 16);
-      f *= rsqrtf(sq / static_cast<float>(2 * DK) + d.norm_eps);
-    }
-    if (!mine) continue;
-#pragma unroll
-    for (int h = 0; h < HV; ++h) {
-      const int dim = 128 * h + 16 * g;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) o[h][k] *= f;
-      if (d.norm_w != nullptr) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) o[h][k] *= load_as_float(d.norm_w, d.norm_dtype, dim + k);
-      }
-      store16_from_float(p.out, p.out_dtype, it.b * p.o_st[0] + head * p.o_st[1] + dim * p.o_st[2], p.o_st[2], o[h],
-                         ring.stage0, lane);
-    }
-  }
+  store_rows<NB, 2 * DK>(prow, ring.stage0, d.group, lane);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -567,12 +725,13 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 template <int DK>
 struct DiffF16Shape {
   static constexpr int kStage = DK * 128;  // 2 tensors x 2 heads x 16 tokens x 2 DK bytes
-  static constexpr int kWarpsPerSm = DK == 128 ? 4 : 8;
-  static constexpr int kStages = 192 * 1024 / (kWarpsPerSm * kStage);
+  static constexpr int kPerSm = DK == 128 ? 4 : 8;
+  static constexpr int kStages = 192 * 1024 / (kPerSm * kStage);
+  static constexpr int kSmem = kStages * (kStage + 8) + 1024;
 };
 
-template <int DK, int NB, bool IS_BF16, bool PLANNED>
-__global__ void __launch_bounds__(kDiffWarpsPerCta * kWarp, DiffF16Shape<DK>::kWarpsPerSm / kDiffWarpsPerCta)
+template <int DK, int NB, bool IS_BF16>
+__global__ void __launch_bounds__(kWarp, DiffF16Shape<DK>::kPerSm)
 diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                 const __grid_constant__ DiffParams d) {
   using Shape = DiffF16Shape<DK>;
@@ -581,21 +740,19 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   constexpr int PIECE = 4096;             // one load: 128 bytes x 16 tokens x 2 heads
   extern __shared__ uint8_t smem_raw[];
   const AttnParams& p = d.a;
-  const int wpc = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x, g = lane >> 2, t = lane & 3;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  TileRing<NST, STAGE, DK / 64> ring;
+  DiffRing<NST, STAGE, DK / 64> ring;
   static_assert(TileRing<NST, STAGE, DK / 64>::PIECE == PIECE, "box of the tensor map");
-  ring.stage0 = smem_base + warp * (NST * STAGE);
-  ring.bar0 = smem_base + wpc * NST * STAGE + warp * (NST * 8);
+  ring.stage0 = smem_base;
+  ring.bar0 = smem_base + NST * STAGE;
   ring.tmK = &tmK;
   ring.tmV = &tmV;
   ItemCoord it;
   float* prow;
-  if (!diff_begin<PLANNED>(d, ring, it, prow, static_cast<int64_t>(blockIdx.x) * wpc + warp, 2, lane)) return;
+  diff_item(d, ring, it, lane, 2);
+  if (!diff_range(d, ring, it, prow, lane, false)) return;
   const int n = it.t1 - it.t0;
-  const int pre = n < NST ? n : NST;
-  for (int i = 0; i < pre; ++i) ring.issue(i);
 
   // Queries as B fragments, rounded to the cache's type: step s covers dims 16s..16s+15; lane (g, t) holds column g,
   // dims 16s+2t, +1 and 16s+8+2t, +1
@@ -643,11 +800,11 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   const int v_tok = r8 + 8 * (mi >> 1), v_chunk = mi & 1;   // V (transposed)
 
   for (int i = 0; i < n; ++i) {
-    if (!ring.wait(i)) {
-      diff_timed_out<NST>(p, ring, i, n, lane);
+    if (!ring.wait_tile(0)) {
+      ring.give_up(p, min(NST, n - i));
       return;
     }
-    const uint32_t kb = ring.stage(i), vb = kb + STAGE / 2;
+    const uint32_t kb = ring.stage_addr(0), vb = kb + STAGE / 2;
     float sm[2][2][4];  // [map's K head][even / odd step]: two chains per head
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -664,30 +821,35 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     }
     const int tile_tok = (it.t0 + i) * kTile;
     const int tok0 = tile_tok + g;
-    uint32_t pb[NB][2];
+    float v[NB][4], f[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      float v[4], f[2];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         // NB = 1: both K heads met all columns, each column keeps its own map's score
         const float own = NB == 1 ? (t < 2 ? sm[0][0][r] + sm[0][1][r] : sm[1][0][r] + sm[1][1][r])
                                   : sm[nb][0][r] + sm[nb][1][r];
-        v[r] = own * p.sm_scale_log2;
+        v[nb][r] = own * p.sm_scale_log2;
       }
-      if (tok0 >= it.seq_len) v[0] = v[1] = -INFINITY;
-      if (tok0 + 8 >= it.seq_len) v[2] = v[3] = -INFINITY;
-      if (softmax_step(st[nb], v, f)) {
+      if (tok0 >= it.seq_len) v[nb][0] = v[nb][1] = -INFINITY;
+      if (tok0 + 8 >= it.seq_len) v[nb][2] = v[nb][3] = -INFINITY;
+    }
+    if (softmax_step<NB, 4>(st, v, f)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int j = 0; j < STEPS; ++j) {
-            acc[h][nb][j][0] *= f[0]; acc[h][nb][j][1] *= f[1]; acc[h][nb][j][2] *= f[0]; acc[h][nb][j][3] *= f[1];
+            acc[h][nb][j][0] *= f[nb][0]; acc[h][nb][j][1] *= f[nb][1]; acc[h][nb][j][2] *= f[nb][0]; acc[h][nb][j][3] *= f[nb][1];
           }
-      }
-      // P^T as B operands, rounded to the cache's type (the sum keeps the unrounded values)
-      pb[nb][0] = movmatrix_trans(pack16<IS_BF16>(v[0], v[1]));
-      pb[nb][1] = movmatrix_trans(pack16<IS_BF16>(v[2], v[3]));
+    }
+    // P^T as B operands, rounded to the cache's type (the sum keeps the unrounded values)
+    uint32_t pb[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      pb[nb][0] = movmatrix_trans(pack16<IS_BF16>(v[nb][0], v[nb][1]));
+      pb[nb][1] = movmatrix_trans(pack16<IS_BF16>(v[nb][2], v[nb][3]));
     }
     // A float cache may hold NaN or infinities behind the last token, and 0 * NaN would poison the sums: those V values
     // are zeroed (their scores were replaced above).
@@ -708,199 +870,183 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) mma16<IS_BF16>(acc[h][nb][j], a, pb[nb][0], pb[nb][1]);
       }
-    __syncwarp();
-    if (i + NST < n) ring.issue(i + NST);
+    ring.advance(1);
   }
 
-  // ---- epilogue: dims DK h + 16 j + g (registers 0, 1) and + 8 (2, 3) of columns 2t and 2t+1 --------------------
+  constexpr int kRow = (2 * DK + 4) * 4;  // bytes of a partial row
+  static_assert(16 * kRow <= NST * STAGE, "the rows of a group fit the ring");
+  // ---- epilogue: dims DK h + 16 j + g (registers 0, 1) and + 8 (2, 3) of columns 2t and 2t+1 -----------
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     reduce_sums(st[nb]);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float inv = inv_sum(st[nb].l[e]);
+      const uint32_t row = ring.stage0 + row_slot<NB>(nb, e, t) * kRow;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
-          acc[h][nb][j][e] *= inv;
-          acc[h][nb][j][e + 2] *= inv;
+          sts32(row + (DK * h + 16 * j + g) * 4, acc[h][nb][j][e]);
+          sts32(row + (DK * h + 16 * j + g + 8) * 4, acc[h][nb][j][e + 2]);
         }
+      if (g == 0) sts128(row + 2 * DK * 4, part_ref(st[nb].m[e], st[nb].l[e]), st[nb].l[e], 0.f, 0.f);
     }
   }
-  if (prow != nullptr) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int hg = col_pair<NB>(2 * t + e), m = col_map<NB>(nb, 2 * t + e);
-        if (hg >= d.group) continue;
-        float* row = prow + (2 * hg + m) * p.row_floats;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < STEPS; ++j) {
-            row[DK * h + 16 * j + g] = acc[h][nb][j][e];
-            row[DK * h + 16 * j + g + 8] = acc[h][nb][j][e + 2];
-          }
-        if (g == 0) row[p.D] = lse_of(st[nb].m[e], st[nb].l[e]);
-      }
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int hg = col_pair<NB>(2 * t + e);
-    const bool mine = hg < d.group && (NB == 2 || t < 2);
-    const int head = it.h * d.group + (mine ? hg : 0);
-    const float lam = load_as_float(d.lam, d.lam_dtype, head * d.lam_st);
-    float o[2][STEPS][2], sq = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float a = acc[h][0][j][e + 2 * k];
-          const float b = NB == 2 ? acc[h][NB - 1][j][e + 2 * k] : __shfl_xor_sync(kFull, a, 2);
-          o[h][j][k] = a - lam * b;
-          sq = fmaf(o[h][j][k], o[h][j][k], sq);
-        }
-    float f = d.out_scale;
-    if (d.norm_w != nullptr) {
-      sq += __shfl_xor_sync(kFull, sq, 4);
-      sq += __shfl_xor_sync(kFull, sq, 8);
-      sq += __shfl_xor_sync(kFull, sq, 16);
-      f *= rsqrtf(sq / static_cast<float>(2 * DK) + d.norm_eps);
-    }
-    if (!mine) continue;
-    const int64_t base = it.b * p.o_st[0] + head * p.o_st[1];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int dim = DK * h + 16 * j + g + 8 * k;
-          const float nw = d.norm_w != nullptr ? load_as_float(d.norm_w, d.norm_dtype, dim) : 1.f;
-          store_from_float(p.out, p.out_dtype, base + dim * p.o_st[2], o[h][j][k] * f * nw);
-        }
-  }
+  store_rows<NB, 2 * DK>(prow, ring.stage0, d.group, lane);
 }
 
 // ---------------------------------------------------------------------------------------------
-// Join of the parts, subtraction, norm: one CTA per (sequence, query pair).
+// Join of the parts, subtraction, norm: one CTA per (sequence, query pair), grid (sequence, pair).
 // ---------------------------------------------------------------------------------------------
-// Thread (group, col) sums 16-byte piece col of the parts group, group + groups, ... of both maps, already weighted
-// with w / den and with -lam for the second map; the groups are added in a fixed order.  Empty parts (log-sum-exp
-// -inf) were never written and are not read.
-constexpr int kDiffMergeThreads = 128;
-static_assert(kDiffMergeThreads >= kMaxSplits, "one thread per part");
+// A short kernel on the critical path of a small call.  The two rows of a part lie side by side and arrive by one bulk copy
+// per part, all parts of a batch in flight at once: ordinary loads, 1024 lines from as many 16-byte pieces, ran at
+// 9 bytes per cycle and SM, limited by the misses that an SM keeps outstanding.  A warp then owns 128 bytes of the row:
+// lane (sub, c) takes 16-byte piece c of the parts sub, sub + 4, ... of both maps; maximum, sum and weighted rows meet
+// in two shuffle steps, and the only CTA barrier is the norm's.  Rows of empty parts (m = -inf) were never
+// written: what is read of them meets no weight.
+constexpr int kMergeBatch = 32;  // parts in shared memory at a time, at most
 
-__global__ void __launch_bounds__(kDiffMergeThreads) diff_merge_kernel(const DiffParams d) {
-  __shared__ float w_s[2][kMaxSplits];
-  __shared__ float4 red_s[kDiffMergeThreads];
-  __shared__ float warp_s[4][2];
+__global__ void __launch_bounds__(512) diff_merge_kernel(const __grid_constant__ DiffParams d, const int batch) {
+  extern __shared__ __align__(16) uint8_t merge_smem[];  // [batch] pairs of rows
+  __shared__ __align__(8) uint64_t bar_s;
+  __shared__ float sq_s[16];
   const AttnParams& p = d.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = static_cast<int>(blockIdx.x / d.heads), h = static_cast<int>(blockIdx.x - static_cast<unsigned>(b) * d.heads);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane >> 3;
+  const int b = blockIdx.x, h = blockIdx.y;
+  const int dim = 32 * warp + 4 * (lane & 7);  // first of this lane's four values
+  const bool live = dim < p.row_floats;
+  const uint32_t rows_s = smem_u32(merge_smem), bar = smem_u32(&bar_s), pair_bytes = 8u * p.row_floats;
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    mbar_fence_init();
+  }
+  // lam, the norm's weights and the scales are inputs of the call: whatever wrote them was complete before the attention kernel let
+  // this one be scheduled
   const float lam = load_as_float(d.lam, d.lam_dtype, h * d.lam_st);
+  float nw[4] = {1.f, 1.f, 1.f, 1.f};
+  if (d.norm_w != nullptr && sub == 0) {
+    if (dim + 3 < p.D) {
+      load4_as_float(d.norm_w, d.norm_dtype, dim, 1, nw);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (dim + u < p.D) nw[u] = load_as_float(d.norm_w, d.norm_dtype, dim + u);
+    }
+  }
+  // V scale of this lane's values, which may straddle the two halves of the row (head dims that are no multiple of 4)
+  float vs[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    vs[u] = p.v_scale != nullptr && dim + u < p.D ? fmaxf(p.v_scale[2 * (h / d.group) + (dim + u >= d.Dk)], 1e-6f) : 1.f;
+  __syncthreads();  // the barrier is initialised
   grid_dependency_wait();
   grid_launch_dependents();
-  int R = p.num_splits;
-  int64_t stride_r = static_cast<int64_t>(p.B) * p.Hq * p.row_floats;
+  const int R = p.num_splits;
+  const int64_t stride_r = static_cast<int64_t>(p.B) * p.Hq * p.row_floats;
   const float* base = p.part + (static_cast<int64_t>(b) * p.Hq + 2 * h) * p.row_floats;
-  if (p.plan_table != nullptr) {  // device-planned parts: consecutive part numbers; a single one went to `out` itself
-    const int2 e = __ldcg(p.plan_table + b);
-    if (e.y <= 1) return;
-    R = e.y < kMaxSplits ? e.y : kMaxSplits;
-    stride_r = static_cast<int64_t>(p.Hq) * p.row_floats;
-    base = p.part + (static_cast<int64_t>(e.x) * p.Hq + 2 * h) * p.row_floats;
-  }
-
-  float lse[2] = {-INFINITY, -INFINITY};
-  if (tid < R) {
-    lse[0] = __ldcg(base + tid * stride_r + p.D);
-    lse[1] = __ldcg(base + tid * stride_r + p.row_floats + p.D);
-  }
-  // block maximum, then block sum, of both maps
-  float top[2], den[2];
+  float4 acc[2];
+  float top[2] = {-INFINITY, -INFINITY}, den[2] = {0.f, 0.f};
+  acc[0] = acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+  uint32_t phase = 0u;
+  for (int r0 = 0; r0 < R; r0 += batch) {
+    const int count = min(batch, R - r0);
+    if (warp == 0) {
+      if (lane == 0) mbar_expect_tx(bar, count * pair_bytes);
+      __syncwarp();
+      for (int r = lane; r < count; r += kWarp)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(rows_s + r * pair_bytes), "l"(base + (r0 + r) * stride_r), "r"(pair_bytes), "r"(bar) : "memory");
+    }
+    if (!__syncthreads_and(mbar_wait_bounded(bar, phase))) {
+      if (tid == 0 && p.status != nullptr) atomicOr(p.status, INT8KV_DEV_WAIT_TIMEOUT);
+      return;
+    }
+    phase ^= 1u;
+    // this lane's (at most eight) parts, both maps side by side
+    float ref[kMergeBatch / 4][2];
+    float t[2] = {top[0], top[1]};
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    float t = lse[m];
-    for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, o));
-    if (lane == 0) warp_s[warp][m] = t;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int m = 0; m < 2; ++m) top[m] = fmaxf(fmaxf(warp_s[0][m], warp_s[1][m]), fmaxf(warp_s[2][m], warp_s[3][m]));
-  __syncthreads();
-  float w[2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    w[m] = lse[m] == -INFINITY ? 0.f : __expf(lse[m] - top[m]);
-    float t = w[m];
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kFull, t, o);
-    if (lane == 0) warp_s[warp][m] = t;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    den[m] = (warp_s[0][m] + warp_s[1][m]) + (warp_s[2][m] + warp_s[3][m]);
-    const float f = den[m] == 0.f ? 0.f : (m == 0 ? 1.f : -lam) / den[m];
-    if (tid < R) w_s[m][tid] = lse[m] == -INFINITY ? 0.f : w[m] * f;
-  }
-  __syncthreads();
-
-  const int cols = (p.D + 3) / 4;  // at most 128
-  const int groups = kDiffMergeThreads / cols;
-  const int group = tid / cols, col = tid - group * cols;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (group < groups) {
-#pragma unroll 4
-    for (int r = group; r < R; r += groups) {
+    for (int u = 0; u < kMergeBatch / 4; ++u)
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const float wr = w_s[m][r];
-        // a part that weighs nothing is not read; lam = 0 switches the second map off (a NaN weight is not zero)
-        if (wr != 0.f) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(base + r * stride_r + m * p.row_floats) + col);
-          a.x += wr * x.x; a.y += wr * x.y; a.z += wr * x.z; a.w += wr * x.w;
+        const int r = sub + 4 * u;
+        ref[u][m] = r < count ? lds32f(rows_s + r * pair_bytes + 4u * (m * p.row_floats + p.D)) : -INFINITY;
+        t[m] = fmaxf(t[m], ref[u][m]);
+      }
+#pragma unroll
+    for (int o = 8; o <= 16; o <<= 1) {  // the four sub-rows of parts share the reference
+      const float a0 = __shfl_xor_sync(kFull, t[0], o), a1 = __shfl_xor_sync(kFull, t[1], o);
+      t[0] = fmaxf(t[0], a0);
+      t[1] = fmaxf(t[1], a1);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if (r0 > 0) {
+        const float f = top[m] == -INFINITY ? 1.f : exp2_fast(top[m] - t[m]);
+        den[m] *= f;
+        acc[m].x *= f; acc[m].y *= f; acc[m].z *= f; acc[m].w *= f;
+      }
+      top[m] = t[m];
+    }
+#pragma unroll
+    for (int u = 0; u < kMergeBatch / 4; ++u) {
+      if (4 * u >= count) break;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        if (ref[u][m] != -INFINITY && live) {
+          const uint32_t row = rows_s + (sub + 4 * u) * pair_bytes + 4u * m * p.row_floats;
+          const float w = exp2_fast(ref[u][m] - t[m]);
+          const uint4 q = lds128(row + 4u * dim);
+          den[m] = fmaf(w, lds32f(row + 4u * p.D + 4u), den[m]);
+          acc[m].x = fmaf(w, __uint_as_float(q.x), acc[m].x); acc[m].y = fmaf(w, __uint_as_float(q.y), acc[m].y);
+          acc[m].z = fmaf(w, __uint_as_float(q.z), acc[m].z); acc[m].w = fmaf(w, __uint_as_float(q.w), acc[m].w);
         }
       }
     }
+    if (r0 + batch < R) __syncthreads();  // the rows are consumed before the next batch lands on them
   }
-  red_s[tid] = a;
-  __syncthreads();
-  float sq = 0.f;
-  if (group == 0) {
-    for (int u = 1; u < groups; ++u) {
-      const float4 x = red_s[u * cols + col];
-      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-    }
-    // the last piece of a row whose length is not a multiple of four ends in the log-sum-exp and padding
-    if (4 * col + 1 >= p.D) a.y = 0.f;
-    if (4 * col + 2 >= p.D) a.z = 0.f;
-    if (4 * col + 3 >= p.D) a.w = 0.f;
-    sq = (a.x * a.x + a.y * a.y) + (a.z * a.z + a.w * a.w);
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    float y[5] = {acc[m].x, acc[m].y, acc[m].z, acc[m].w, den[m]};
+#pragma unroll
+    for (int u = 0; u < 5; ++u) y[u] += __shfl_xor_sync(kFull, y[u], 8);
+#pragma unroll
+    for (int u = 0; u < 5; ++u) y[u] += __shfl_xor_sync(kFull, y[u], 16);
+    const float f = y[4] == 0.f ? 0.f : (m == 0 ? 1.f : -lam) / y[4];  // a NaN sum stays one
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = fmaf(f, y[u], v[u]);
   }
+  // what lies behind the row's values (m, l, padding) is not part of the norm
+#pragma unroll
+  for (int u = 0; u < 4; ++u) v[u] = dim + u < p.D ? v[u] * vs[u] : 0.f;
   float f = d.out_scale;
   if (d.norm_w != nullptr) {
-    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(kFull, sq, o);
-    if (lane == 0) warp_s[warp][0] = sq;
+    float sq = (v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]);
+    sq += __shfl_xor_sync(kFull, sq, 1);  // over the eight pieces
+    sq += __shfl_xor_sync(kFull, sq, 2);
+    sq += __shfl_xor_sync(kFull, sq, 4);
+    if (lane == 0) sq_s[warp] = sq;
     __syncthreads();
-    sq = (warp_s[0][0] + warp_s[1][0]) + (warp_s[2][0] + warp_s[3][0]);
+    sq = 0.f;
+    for (int u = 0; u < static_cast<int>(blockDim.x) / kWarp; ++u) sq += sq_s[u];
     f *= rsqrtf(sq / static_cast<float>(p.D) + d.norm_eps);
   }
-  if (group != 0) return;
-  const float v[4] = {a.x, a.y, a.z, a.w};
-  const int64_t ob = b * p.o_st[0] + h * p.o_st[1];
+  if (sub != 0 || dim >= p.D) return;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int dd = 4 * col + u;
-    if (dd >= p.D) break;
-    const float nw = d.norm_w != nullptr ? load_as_float(d.norm_w, d.norm_dtype, dd) : 1.f;
-    store_from_float(p.out, p.out_dtype, ob + dd * p.o_st[2], v[u] * f * nw);
+  for (int u = 0; u < 4; ++u) v[u] *= f * nw[u];
+  const int64_t ob = b * p.o_st[0] + h * p.o_st[1], at = ob + dim;
+  if (p.out_dtype != INT8KV_FP32 && p.o_st[2] == 1 && dim + 3 < p.D &&
+      ((reinterpret_cast<uintptr_t>(p.out) + 2 * at) & 7u) == 0) {
+    uint2 word;
+    word.x = p.out_dtype == INT8KV_BF16 ? pack_bf162(v[0], v[1]) : pack_half2(v[0], v[1]);
+    word.y = p.out_dtype == INT8KV_BF16 ? pack_bf162(v[2], v[3]) : pack_half2(v[2], v[3]);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = word;
+    return;
   }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (dim + u < p.D) store_from_float(p.out, p.out_dtype, ob + (dim + u) * p.o_st[2], v[u]);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -938,50 +1084,45 @@ static bool raise_smem(size_t bytes) {
 }
 
 template <auto KERNEL, typename Shape>
-static int launch_diff_shape(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, int sm_count, cudaStream_t stream) {
-  constexpr int per_warp = Shape::kStages * (Shape::kStage + 8);
-  if (!raise_smem<KERNEL>(kDiffWarpsPerCta * per_warp + 1024)) return INT8KV_E_LAUNCH;
+static int launch_diff_shape(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t stream) {
+  if (!raise_smem<KERNEL>(Shape::kSmem)) return INT8KV_E_LAUNCH;
   const AttnParams& p = d.a;
-  const int64_t items = p.plan_table != nullptr ? p.plan_grid_items : static_cast<int64_t>(p.B) * p.num_splits * p.Hkv;
+  const int64_t items = static_cast<int64_t>(p.B) * p.num_splits * p.Hkv;
   if (items >= (int64_t(1) << 31)) return INT8KV_E_UNSUPPORTED;  // the kernels number their items in 32 bits
-  // a grid that does not fill the machine with four-warp CTAs runs as one-warp CTAs, spread over all SMs
-  const int wpc = items <= static_cast<int64_t>(sm_count) * Shape::kWarpsPerSm ? 1 : kDiffWarpsPerCta;
-  return launch_pdl(KERNEL, static_cast<unsigned>((items + wpc - 1) / wpc), wpc * kWarp,
-                    static_cast<size_t>(wpc) * per_warp + 1024, stream, tmK, tmV, d);
+  return launch_pdl(KERNEL, static_cast<unsigned>(items), kWarp, Shape::kSmem, stream, tmK, tmV, d);
 }
 
 template <int DK, int NB>
-static int launch_diff_tiled_shape(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, int sm_count,
-                                   cudaStream_t stream) {
-  const bool planned = d.a.plan_table != nullptr;
+static int launch_diff_tiled_shape(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t stream) {
   if (d.a.cache_kind == kCacheInt8)
-    return planned ? launch_diff_shape<diff_int8_kernel<DK, NB, true>, DiffInt8Shape<DK, NB>>(d, tmK, tmV, sm_count, stream)
-                   : launch_diff_shape<diff_int8_kernel<DK, NB, false>, DiffInt8Shape<DK, NB>>(d, tmK, tmV, sm_count, stream);
+    return launch_diff_shape<diff_int8_kernel<DK, NB>, DiffInt8Shape<DK, NB>>(d, tmK, tmV, stream);
   if (d.a.cache_kind == kCacheBf16)
-    return planned ? launch_diff_shape<diff_f16_kernel<DK, NB, true, true>, DiffF16Shape<DK>>(d, tmK, tmV, sm_count, stream)
-                   : launch_diff_shape<diff_f16_kernel<DK, NB, true, false>, DiffF16Shape<DK>>(d, tmK, tmV, sm_count, stream);
-  return planned ? launch_diff_shape<diff_f16_kernel<DK, NB, false, true>, DiffF16Shape<DK>>(d, tmK, tmV, sm_count, stream)
-                 : launch_diff_shape<diff_f16_kernel<DK, NB, false, false>, DiffF16Shape<DK>>(d, tmK, tmV, sm_count, stream);
+    return launch_diff_shape<diff_f16_kernel<DK, NB, true>, DiffF16Shape<DK>>(d, tmK, tmV, stream);
+  return launch_diff_shape<diff_f16_kernel<DK, NB, false>, DiffF16Shape<DK>>(d, tmK, tmV, stream);
 }
 
-int diff_warps_per_sm(int cache_kind, int D, int group) {
-  if (cache_kind != kCacheInt8) return D == 128 ? DiffF16Shape<128>::kWarpsPerSm : DiffF16Shape<64>::kWarpsPerSm;
-  if (D == 128) return group <= 4 ? DiffInt8Shape<128, 1>::kWarpsPerSm : DiffInt8Shape<128, 2>::kWarpsPerSm;
-  return group <= 4 ? DiffInt8Shape<64, 1>::kWarpsPerSm : DiffInt8Shape<64, 2>::kWarpsPerSm;
+int diff_items_per_sm(int cache_kind, int D, int group) {
+  if (cache_kind != kCacheInt8) return D == 128 ? DiffF16Shape<128>::kPerSm : DiffF16Shape<64>::kPerSm;
+  if (D == 128) return group <= 4 ? DiffInt8Shape<128, 1>::kPerSm : DiffInt8Shape<128, 2>::kPerSm;
+  return group <= 4 ? DiffInt8Shape<64, 1>::kPerSm : DiffInt8Shape<64, 2>::kPerSm;
 }
 
-int launch_diff_tiled(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, int sm_count, cudaStream_t stream) {
+int launch_diff_tiled(const DiffParams& d, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t stream) {
   if (d.Dk == 128)
-    return d.group <= 4 ? launch_diff_tiled_shape<128, 1>(d, tmK, tmV, sm_count, stream)
-                        : launch_diff_tiled_shape<128, 2>(d, tmK, tmV, sm_count, stream);
-  return d.group <= 4 ? launch_diff_tiled_shape<64, 1>(d, tmK, tmV, sm_count, stream)
-                      : launch_diff_tiled_shape<64, 2>(d, tmK, tmV, sm_count, stream);
+    return d.group <= 4 ? launch_diff_tiled_shape<128, 1>(d, tmK, tmV, stream)
+                        : launch_diff_tiled_shape<128, 2>(d, tmK, tmV, stream);
+  return d.group <= 4 ? launch_diff_tiled_shape<64, 1>(d, tmK, tmV, stream)
+                      : launch_diff_tiled_shape<64, 2>(d, tmK, tmV, stream);
 }
 
 int launch_diff_merge(const DiffParams& d, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(d.a.B) * d.heads;
-  if (rows >= (int64_t(1) << 31)) return INT8KV_E_UNSUPPORTED;
-  return launch_pdl(diff_merge_kernel, static_cast<unsigned>(rows), kDiffMergeThreads, 0, stream, d);
+  const AttnParams& p = d.a;
+  if (d.heads > 65535) return INT8KV_E_UNSUPPORTED;  // grid y
+  const int batch = std::min(kMergeBatch, p.num_splits);
+  if (!raise_smem<diff_merge_kernel>(kMergeBatch * 8 * (2 * kDiffMaxD + 4))) return INT8KV_E_LAUNCH;
+  const unsigned warps = static_cast<unsigned>((p.D + 31) / 32);  // at most 16
+  return launch_pdl(diff_merge_kernel, dim3(static_cast<unsigned>(p.B), static_cast<unsigned>(d.heads), 1), warps * kWarp,
+                    static_cast<size_t>(batch) * 8 * p.row_floats, stream, d, batch);
 }
 
 }  // namespace int8kv

@@ -164,6 +164,30 @@ def test_large_magnitudes(kv):
         verify(kv, c)
 
 
+def test_maps_of_different_size(kv):
+    """Queries of the two maps, and of the heads of a group, four orders of magnitude apart: each head has its own scale."""
+    for D, heads in ((128, 4), (128, 7), (64, 4), (64, 7)):
+        for small in (0, 1):
+            c = make_case(21, [150, 31], heads, 1, D, 16, torch.int8, sharp=2.0)
+            c["q"][:, small::2] *= 1e-4
+            c["q"][:, 2] *= 30
+            c["ks"][small::2] *= 1e4  # the scores of the small queries matter all the same
+            verify(kv, c)
+
+
+def test_bad_values_stay_in_their_head(kv):
+    """A NaN or an infinity in one query head reaches that differential head only."""
+    for cache in (torch.int8, torch.bfloat16):
+        for D, heads in ((128, 4), (128, 7), (64, 4), (64, 7), (40, 3)):
+            c = make_case(22, [150, 31], heads, 1, D, 16, cache)
+            want = call(kv, c)
+            c["q"][0, 3, 5] = float("nan")
+            got = call(kv, c)
+            assert torch.isnan(got[0, 1]).all()
+            got[0, 1] = want[0, 1]
+            assert torch.equal(got, want)
+
+
 def test_equal_maps_cancel(kv):
     """The same queries and keys in both maps and lam = 1: what is left is rounding, whatever the length."""
     for D in (128, 64):
