@@ -185,72 +185,64 @@ __device__ __forceinline__ int col_map(int nb, int c) { return NB == 1 ? c >> 2 
 template <int NB>
 __device__ __forceinline__ int col_pair(int c) { return NB == 1 ? c & 3 : c; }
 
-// Running softmax of the columns of one block: reference exponent and sum of columns 2t (index 0) and 2t+1.  The reference
-// m is a score that was the column's maximum when it was set; it follows the maximum only when that has moved more than
-// kSlack (in log2 units) above it, so probabilities reach up to 2^kSlack, which fp16, bf16 and the fp32 sums hold with the
-// same relative precision as values up to 1.  A step then needs no reduction across the token lanes, just a vote, and
-// the accumulators are rescaled a few times per part instead of in every other tile (measured on 32 x 32k tokens, groups
-// of 8: see the kernel).
+// Running softmax of the columns of one block: reference m of columns 2t (index 0) and 2t+1, in log2 units.  It is a score
+// that was the column's maximum when it was set, and follows the maximum only when that has moved more than kSlack above
+// it: probabilities reach up to 2^kSlack, which fp16, bf16 and the fp32 sums hold with the same relative precision as
+// values up to 1.  A step then needs no reduction across the token lanes, just a vote, and the accumulators are rescaled a
+// few times per part instead of in every other tile (32 x 32k tokens, groups of eight: 324 -> 309 us).
 constexpr float kSlack = 8.f;
-struct ColStats {
-  float m[2], l[2];
-};
 
-// One online-softmax step over NV / 2 score rows per lane and NB column blocks at once (log2 units; v[nb][2k], v[nb][2k+1]
-// are columns 2t, 2t+1 of a row): v becomes the probabilities relative to the references; returns whether the
-// accumulators have to follow, by f[nb][0], f[nb][1].
+// One online-softmax step over NV / 2 score rows per lane and NB column blocks at once.  x: scores before the factors
+// sc, x[nb][2k] and x[nb][2k+1] being columns 2t and 2t+1 of token row g + 8k, of which the first `valid` count.  x becomes
+// the probabilities 2^(x sc - m); returns whether m moved, and with it the accumulators, by f[nb][0], f[nb][1].
 template <int NB, int NV>
-__device__ __forceinline__ bool softmax_step(ColStats (&s)[NB], float (&v)[NB][NV], float (&f)[NB][2]) {
-  float mx[NB][2];
-  bool high = false;
+__device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][NV], const float (&sc)[NB][2], float (&f)[NB][2],
+                                             int valid, int g) {
+  float y[NB][NV];
+  float top = -INFINITY;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      mx[nb][e] = v[nb][e];
+    for (int k = 0; k < NV; ++k) y[nb][k] = fmaf(x[nb][k], sc[nb][k & 1], -m[nb][k & 1]);
+  if (valid < 4 * NV) {  // the sequence's last tile (NV / 2 rows of 8 tokens)
 #pragma unroll
-      for (int k = 2 + e; k < NV; k += 2) mx[nb][e] = fmaxf(mx[nb][e], v[nb][k]);
-      high = high || mx[nb][e] > s[nb].m[e] + kSlack;
-    }
-  const bool moved = __any_sync(kFull, high);
+    for (int k = 0; k < NV; ++k)
+      if (g + 8 * (k >> 1) >= valid) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) y[nb][k] = -INFINITY;
+      }
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) top = fmaxf(top, y[nb][k]);
+  const bool moved = __any_sync(kFull, top > kSlack);  // also while m is -inf: y is +inf then
   if (moved) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = mx[nb][e];
-        x = fmaxf(x, __shfl_xor_sync(kFull, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(kFull, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(kFull, x, 16));
-        x = fmaxf(x, s[nb].m[e]);
-        f[nb][e] = x == s[nb].m[e] ? 1.f : exp2_fast(s[nb].m[e] - x);  // equal also when nothing but -inf was seen
-        s[nb].l[e] *= f[nb][e];
-        s[nb].m[e] = x;
+        float z = -INFINITY;
+#pragma unroll
+        for (int k = e; k < NV; k += 2) {
+          y[nb][k] = g + 8 * (k >> 1) < valid ? x[nb][k] * sc[nb][e] : -INFINITY;
+          z = fmaxf(z, y[nb][k]);
+        }
+        z = fmaxf(z, __shfl_xor_sync(kFull, z, 4));
+        z = fmaxf(z, __shfl_xor_sync(kFull, z, 8));
+        z = fmaxf(z, __shfl_xor_sync(kFull, z, 16));
+        z = fmaxf(z, m[nb][e]);
+        f[nb][e] = z == m[nb][e] ? 1.f : exp2_fast(m[nb][e] - z);  // equal also when nothing but -inf was seen
+        m[nb][e] = z;
+#pragma unroll
+        for (int k = e; k < NV; k += 2) y[nb][k] -= z;
       }
   }
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int k = 0; k < NV; ++k) v[nb][k] = exp2_fast(v[nb][k] - s[nb].m[k & 1]);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float sum = v[nb][e];
-#pragma unroll
-      for (int k = 2 + e; k < NV; k += 2) sum += v[nb][k];
-      s[nb].l[e] += sum;
-    }
-  }
+    for (int k = 0; k < NV; ++k) x[nb][k] = exp2_fast(y[nb][k]);
   return moved;
-}
-
-// Row sums over the token lanes.
-__device__ __forceinline__ void reduce_sums(ColStats& s) {
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    s.l[e] += __shfl_xor_sync(kFull, s.l[e], 4);
-    s.l[e] += __shfl_xor_sync(kFull, s.l[e], 8);
-    s.l[e] += __shfl_xor_sync(kFull, s.l[e], 16);
-  }
 }
 
 // The ring of one item: tiles are issued and consumed in order, so stage, phase, block and tile-in-block are counters
@@ -446,26 +438,29 @@ __device__ __forceinline__ void store_rows(float* prow, uint32_t slots, int grou
 __device__ __forceinline__ void sts128(uint32_t addr, float a, float b, float c, float e) {
   asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(e) : "memory");
 }
+__device__ __forceinline__ void sts64(uint32_t addr, float a, float b) {
+  asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+}
 __device__ __forceinline__ void sts32(uint32_t addr, float a) {
   asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(a) : "memory");
 }
 
-// Eight dims x 16 tokens of V^T per step, INT8 -> fp16 on the way (see pv_tile), times P^T of NB column blocks.
+// One V tile (16 tokens x 128 values, INT8) times P^T of NB column blocks.  ldmatrix transposes 16-bit units: lane (g, t)
+// receives the bytes of values 2g, 2g+1 of a 16-value chunk for tokens 2t and 2t+1 in one register, from which one byte
+// permute each makes the two rows of the MMA's A operand (row g = value 2g, row g + 8 = value 2g + 1), as 1024 + (v + 128)
+// in fp16; the subtraction of 1152 is exact.
 template <int NB>
-__device__ __forceinline__ void pv_blocks(float (&acc)[NB][8][4], const uint4 (&vx)[4], const uint32_t (&pb)[NB][2]) {
-  const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vx[0]);
-  const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vx[1]);
-  const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vx[2]);
-  const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vx[3]);
+__device__ __forceinline__ void pv_blocks(float (&acc)[NB][8][4], uint32_t tile, const uint32_t (&voff)[4], const uint32_t (&pb)[NB][2]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const uint32_t x0 = w0[c] ^ 0x80808080u, x1 = w1[c] ^ 0x80808080u;
-    const uint32_t x2 = w2[c] ^ 0x80808080u, x3 = w3[c] ^ 0x80808080u;
+  for (int c = 0; c < 4; ++c) {  // two chunks
+    uint32_t w[4];
+    ldmatrix_x4_trans(w, tile + voff[c]);  // {tokens 0-7, 8-15} of chunk 2c, then of chunk 2c + 1
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] ^= 0x80808080u;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const uint32_t a01 = prmt(x0, x1, s == 0 ? 0x5140u : 0x7362u), a23 = prmt(x2, x3, s == 0 ? 0x5140u : 0x7362u);
-      const uint32_t f0 = u8pair_to_half2(a01, 0x4140u), f1 = u8pair_to_half2(a01, 0x4342u);
-      const uint32_t f2 = u8pair_to_half2(a23, 0x4140u), f3 = u8pair_to_half2(a23, 0x4342u);
+      const uint32_t f0 = u8pair_to_half2(w[2 * s], 0x4240u), f1 = u8pair_to_half2(w[2 * s], 0x4341u);
+      const uint32_t f2 = u8pair_to_half2(w[2 * s + 1], 0x4240u), f3 = u8pair_to_half2(w[2 * s + 1], 0x4341u);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) mma_f16(acc[nb][2 * c + s], f0, f1, f2, f3, pb[nb][0], pb[nb][1]);
     }
@@ -632,18 +627,24 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
   }
 
   const uint32_t koff[4] = {swz128(g, 2 * t), swz128(g, 2 * t + 1), swz128(g + 8, 2 * t), swz128(g + 8, 2 * t + 1)};
-  const uint32_t voff[4] = {swz128(2 * t, g), swz128(2 * t + 1, g), swz128(2 * t + 8, g), swz128(2 * t + 9, g)};
-  float acc[HV][NB][8][4];
-  ColStats st[NB];
+  // ldmatrix lane roles in a V tile: matrix lane / 8 = (tokens 0-7 / 8-15, chunk 2c / 2c + 1), row lane % 8
+  uint32_t voff[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) voff[c] = swz128((lane & 7) + 8 * ((lane >> 3) & 1), 2 * c + (lane >> 4));
+  // The columns' sums are a row of the P.V product too, with ones for V: they then hold what was multiplied, P as rounded
+  // to fp16, whose error cancels where one token carries the softmax, and need no reduction at the end.
+  constexpr uint32_t kOnes = 0x3c003c00u;
+  float acc[HV][NB][8][4], sum[NB][4], m[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    st[nb].m[0] = st[nb].m[1] = -INFINITY;
-    st[nb].l[0] = st[nb].l[1] = 0.f;
+    m[nb][0] = m[nb][1] = -INFINITY;
+    sum[nb][0] = sum[nb][1] = sum[nb][2] = sum[nb][3] = 0.f;
 #pragma unroll
     for (int h = 0; h < HV; ++h)
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[h][nb][j][0] = acc[h][nb][j][1] = acc[h][nb][j][2] = acc[h][nb][j][3] = 0.f;
   }
+  const int limit = min(it.seq_len, it.t1 * kTile) - it.t0 * kTile;  // tokens of the range
 
   // When the range holds an odd number of tiles the last trip of two has one all masked tile; its stage holds finite
   // integers, stale or fresh, that meet p = 0.
@@ -654,68 +655,57 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
       ring.give_up(p, min(NST, n - i));
       return;
     }
-    float v[NB][4 * TRIP], f[NB][2];
+    float x[NB][4 * TRIP], f[NB][2];
 #pragma unroll
     for (int u = 0; u < TRIP; ++u) {
       int raw[NB][4];
       diff_scores<DK, NB>(raw, ring.stage_addr(u), koff, qh, ql, t);
-      const int tok = (it.t0 + i + u) * kTile + g;
-      const bool in_lo = i + u < n && tok < it.seq_len, in_hi = i + u < n && tok + 8 < it.seq_len;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[nb][4 * u + r] = (r < 2 ? in_lo : in_hi) ? static_cast<float>(raw[nb][r]) * sc[nb][r & 1] : -INFINITY;
+        for (int r = 0; r < 4; ++r) x[nb][4 * u + r] = static_cast<float>(raw[nb][r]);
     }
-    if (softmax_step<NB, 4 * TRIP>(st, v, f)) {
+    if (softmax_step<NB, 4 * TRIP>(m, x, sc, f, limit - i * kTile, g)) {
 #pragma unroll
-      for (int h = 0; h < HV; ++h)
+      for (int nb = 0; nb < NB; ++nb) {
+        sum[nb][0] *= f[nb][0]; sum[nb][1] *= f[nb][1];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int h = 0; h < HV; ++h)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             acc[h][nb][j][0] *= f[nb][0]; acc[h][nb][j][1] *= f[nb][1]; acc[h][nb][j][2] *= f[nb][0]; acc[h][nb][j][3] *= f[nb][1];
           }
+      }
     }
-    // P^T as B operands, rounded to fp16 (the sum keeps the unrounded values)
-    uint32_t pb[TRIP][NB][2];
 #pragma unroll
-    for (int u = 0; u < TRIP; ++u)
+    for (int u = 0; u < TRIP; ++u) {
+      uint32_t pb[NB][2];  // P^T as B operands
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        pb[u][nb][0] = movmatrix_trans(pack_half2(v[nb][4 * u], v[nb][4 * u + 1]));
-        pb[u][nb][1] = movmatrix_trans(pack_half2(v[nb][4 * u + 2], v[nb][4 * u + 3]));
+        pb[nb][0] = movmatrix_trans(pack_half2(x[nb][4 * u], x[nb][4 * u + 1]));
+        pb[nb][1] = movmatrix_trans(pack_half2(x[nb][4 * u + 2], x[nb][4 * u + 3]));
+        mma_f16(sum[nb], kOnes, kOnes, kOnes, kOnes, pb[nb][0], pb[nb][1]);
       }
 #pragma unroll
-    for (int h = 0; h < HV; ++h)
-#pragma unroll
-      for (int u = 0; u < TRIP; ++u) {
-        uint4 vx[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vx[r] = lds128(ring.stage_addr(u) + STAGE / 2 + h * 2048 + voff[r]);
-        pv_blocks<NB>(acc[h], vx, pb[u]);
-      }
+      for (int h = 0; h < HV; ++h) pv_blocks<NB>(acc[h], ring.stage_addr(u) + STAGE / 2 + h * 2048, voff, pb);
+    }
     ring.advance(TRIP);
   }
 
-  // ---- epilogue: lane (g, t) holds dims 128 h + 16 g .. + 15 of columns 2t and 2t+1 ---------------------------
+  // ---- epilogue: lane (g, t) holds values 128 h + 16 j + 2g, + 1 of columns 2t and 2t+1 ---------------------------
   constexpr int kRow = (2 * DK + 4) * 4;  // bytes of a partial row
-  static_assert(16 * kRow <= NST * STAGE, "the rows of a group fit the ring");
+  static_assert(8 * NB * kRow <= NST * STAGE, "the rows of a group fit the ring");
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    reduce_sums(st[nb]);
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {  // (columns without a query pair write slots that are not copied out)
       const uint32_t row = ring.stage0 + row_slot<NB>(nb, e, t) * kRow;
 #pragma unroll
       for (int h = 0; h < HV; ++h)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          sts128(row + (128 * h + 16 * g + 4 * k) * 4, acc[h][nb][2 * k][e], acc[h][nb][2 * k][e + 2], acc[h][nb][2 * k + 1][e],
-                 acc[h][nb][2 * k + 1][e + 2]);
-      if (g == 0) sts128(row + 2 * DK * 4, part_ref(st[nb].m[e], st[nb].l[e]), st[nb].l[e], 0.f, 0.f);
+        for (int j = 0; j < 8; ++j) sts64(row + (128 * h + 16 * j + 2 * g) * 4, acc[h][nb][j][e], acc[h][nb][j][e + 2]);
+      if (g == 0) sts128(row + 2 * DK * 4, part_ref(m[nb][e], sum[nb][e]), sum[nb][e], 0.f, 0.f);
     }
-  }
   store_rows<NB, 2 * DK>(prow, ring.stage0, d.group, lane);
 }
 
@@ -759,8 +749,8 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   uint32_t qf[NB][2 * STEPS];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int m = col_map<NB>(nb, g), hg = col_pair<NB>(g);
-    const int64_t base = it.b * p.q_st[0] + (2 * (it.h * d.group + hg) + m) * p.q_st[1];
+    const int map = col_map<NB>(nb, g), hg = col_pair<NB>(g);
+    const int64_t base = it.b * p.q_st[0] + (2 * (it.h * d.group + hg) + map) * p.q_st[1];
     const bool same_type = p.q_dtype == (IS_BF16 ? INT8KV_BF16 : INT8KV_FP16) && p.q_st[2] == 1 &&
                            ((reinterpret_cast<uintptr_t>(p.q) + 2 * base) & 3u) == 0;
     if (hg >= d.group) {
@@ -783,12 +773,13 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     }
   }
 
-  float acc[2][NB][STEPS][4];
-  ColStats st[NB];
+  constexpr uint32_t kOnes = IS_BF16 ? 0x3f803f80u : 0x3c003c00u;  // the columns' sums as a row of the product, see above
+  float acc[2][NB][STEPS][4], sum[NB][4], m[NB][2], sc[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    st[nb].m[0] = st[nb].m[1] = -INFINITY;
-    st[nb].l[0] = st[nb].l[1] = 0.f;
+    m[nb][0] = m[nb][1] = -INFINITY;
+    sc[nb][0] = sc[nb][1] = p.sm_scale_log2;
+    sum[nb][0] = sum[nb][1] = sum[nb][2] = sum[nb][3] = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -807,53 +798,47 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const uint32_t kb = ring.stage_addr(0), vb = kb + STAGE / 2;
     float sm[2][2][4];  // [map's K head][even / odd step]: two chains per head
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sm[m][0][r] = sm[m][1][r] = 0.f;
-      const int nb = NB == 1 ? 0 : m;
+      for (int r = 0; r < 4; ++r) sm[k][0][r] = sm[k][1][r] = 0.f;
+      const int nb = NB == 1 ? 0 : k;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         const int ch = 2 * s + k_chunk;  // 16-byte chunk of the row
         uint32_t a[4];
-        ldmatrix_x4(a, kb + (ch >> 3) * PIECE + m * 2048 + swz128(k_tok, ch & 7));
-        mma16<IS_BF16>(sm[m][s & 1], a, qf[nb][2 * s], qf[nb][2 * s + 1]);
+        ldmatrix_x4(a, kb + (ch >> 3) * PIECE + k * 2048 + swz128(k_tok, ch & 7));
+        mma16<IS_BF16>(sm[k][s & 1], a, qf[nb][2 * s], qf[nb][2 * s + 1]);
       }
     }
-    const int tile_tok = (it.t0 + i) * kTile;
-    const int tok0 = tile_tok + g;
-    float v[NB][4], f[NB][2];
+    const int nvalid = it.seq_len - (it.t0 + i) * kTile;  // >= 1
+    float x[NB][4], f[NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        // NB = 1: both K heads met all columns, each column keeps its own map's score
-        const float own = NB == 1 ? (t < 2 ? sm[0][0][r] + sm[0][1][r] : sm[1][0][r] + sm[1][1][r])
-                                  : sm[nb][0][r] + sm[nb][1][r];
-        v[nb][r] = own * p.sm_scale_log2;
-      }
-      if (tok0 >= it.seq_len) v[nb][0] = v[nb][1] = -INFINITY;
-      if (tok0 + 8 >= it.seq_len) v[nb][2] = v[nb][3] = -INFINITY;
-    }
-    if (softmax_step<NB, 4>(st, v, f)) {
+      for (int r = 0; r < 4; ++r)  // NB = 1: both K heads met all columns, each column keeps its own map's score
+        x[nb][r] = NB == 1 ? (t < 2 ? sm[0][0][r] + sm[0][1][r] : sm[1][0][r] + sm[1][1][r]) : sm[nb][0][r] + sm[nb][1][r];
+    if (softmax_step<NB, 4>(m, x, sc, f, nvalid, g)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int nb = 0; nb < NB; ++nb) {
+        sum[nb][0] *= f[nb][0]; sum[nb][1] *= f[nb][1];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < STEPS; ++j) {
             acc[h][nb][j][0] *= f[nb][0]; acc[h][nb][j][1] *= f[nb][1]; acc[h][nb][j][2] *= f[nb][0]; acc[h][nb][j][3] *= f[nb][1];
           }
+      }
     }
-    // P^T as B operands, rounded to the cache's type (the sum keeps the unrounded values)
-    uint32_t pb[NB][2];
+    uint32_t pb[NB][2];  // P^T as B operands, rounded to the cache's type
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      pb[nb][0] = movmatrix_trans(pack16<IS_BF16>(v[nb][0], v[nb][1]));
-      pb[nb][1] = movmatrix_trans(pack16<IS_BF16>(v[nb][2], v[nb][3]));
+      pb[nb][0] = movmatrix_trans(pack16<IS_BF16>(x[nb][0], x[nb][1]));
+      pb[nb][1] = movmatrix_trans(pack16<IS_BF16>(x[nb][2], x[nb][3]));
+      const uint32_t ones[4] = {kOnes, kOnes, kOnes, kOnes};
+      mma16<IS_BF16>(sum[nb], ones, pb[nb][0], pb[nb][1]);
     }
     // A float cache may hold NaN or infinities behind the last token, and 0 * NaN would poison the sums: those V values
     // are zeroed (their scores were replaced above).
-    const int nvalid = it.seq_len - tile_tok;  // >= 1
     uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;  // masks for (tokens 2t, 2t+1) and (2t+8, 2t+9)
     if (nvalid < kTile) {
       keep_lo = (2 * t < nvalid ? 0x0000ffffu : 0u) | (2 * t + 1 < nvalid ? 0xffff0000u : 0u);
@@ -874,11 +859,10 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   }
 
   constexpr int kRow = (2 * DK + 4) * 4;  // bytes of a partial row
-  static_assert(16 * kRow <= NST * STAGE, "the rows of a group fit the ring");
-  // ---- epilogue: dims DK h + 16 j + g (registers 0, 1) and + 8 (2, 3) of columns 2t and 2t+1 -----------
+  static_assert(8 * NB * kRow <= NST * STAGE, "the rows of a group fit the ring");
+  // ---- epilogue: values DK h + 16 j + g (registers 0, 1) and + 8 (2, 3) of columns 2t and 2t+1 --------------------
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    reduce_sums(st[nb]);
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t row = ring.stage0 + row_slot<NB>(nb, e, t) * kRow;
@@ -889,9 +873,8 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
           sts32(row + (DK * h + 16 * j + g) * 4, acc[h][nb][j][e]);
           sts32(row + (DK * h + 16 * j + g + 8) * 4, acc[h][nb][j][e + 2]);
         }
-      if (g == 0) sts128(row + 2 * DK * 4, part_ref(st[nb].m[e], st[nb].l[e]), st[nb].l[e], 0.f, 0.f);
+      if (g == 0) sts128(row + 2 * DK * 4, part_ref(m[nb][e], sum[nb][e]), sum[nb][e], 0.f, 0.f);
     }
-  }
   store_rows<NB, 2 * DK>(prow, ring.stage0, d.group, lane);
 }
 

@@ -14,11 +14,12 @@ def diff_paged_attention(query, key_cache, value_cache, block_tables, seq_lens, 
 
     The bound, without the rounding of the output itself: the operator may hold each query head as 16-bit fixed point
     over its largest element (step amax / 32000, off by at most half of it), or round it to the cache's 16-bit type
-    (2^-8 relative for bf16, of which fp16's 2^-11 is a part), and each probability as a 16-bit float (2^-11
-    relative for fp16, 2^-8 for a bf16 cache, the sum being kept unrounded).  A score moves by at most
-    ds = max_n sum_d |dq_d k_nd| / sqrt(D); with it every weight by a factor within exp(+-ds), numerator and
-    denominator both, and a map's output by (2 ds + dp) sum_n p_n |v_n|; fp32 sums, exponentials and divisions add less
-    than 2^-14 of the same.  The norm divides by the row's root mean square r and moves with it, which at most doubles
+    (2^-8 relative for bf16, of which fp16's 2^-11 is a part), and each probability as a 16-bit float (dp = 2^-11
+    relative for fp16, 2^-8 for a bf16 cache), in the product and in the sum it is divided by alike.  A score moves by at
+    most ds = max_n sum_d |dq_d k_nd| / sqrt(D); with it every weight by a factor within exp(+-ds), numerator and
+    denominator both, and a map's output by 2 ds sum_n p_n |v_n|.  Rounded weights p (1 + e), |e| <= dp, move
+    o = sum p v / sum p by at most dp sum p |v - o| <= 2 dp sum p |v| (normalised p).  fp32 sums, exponentials and
+    divisions add less than 2^-14 of the same.  The norm divides by the row's root mean square r and moves with it, which at most doubles
     a relative error.
     """
     B, H2, D = query.shape
@@ -50,7 +51,7 @@ def diff_paged_attention(query, key_cache, value_cache, block_tables, seq_lens, 
                 ds = float((k[:, 2 * g + m].abs() @ dq).amax()) / math.sqrt(D)
                 f = 1.0 if m == 0 else float(lam[h])
                 out[b, h] += (1.0 if m == 0 else -1.0) * f * (p @ v[:, g])
-                bound[b, h] += abs(f) * math.exp(2 * ds) * (2 * ds + dp + 2.0 ** -14) * (p @ v[:, g].abs())
+                bound[b, h] += abs(f) * math.exp(2 * ds) * (2 * ds + 2 * dp + 2.0 ** -14) * (p @ v[:, g].abs())
     bound *= abs(out_scale)
     scaled = out * out_scale
     if norm_weight is not None:
