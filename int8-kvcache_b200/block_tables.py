@@ -41,7 +41,8 @@ def _check_lists(block_tables, seq_lens, block_size):
     assert device.type == "cuda" and block_tables.ndim == 2 and seq_lens.ndim == 1 and seq_lens.device == device
     requests, width = block_tables.shape
     bt_code, sl_code = _INDEX_CODES.get(block_tables.dtype), _INDEX_CODES.get(seq_lens.dtype)
-    assert bt_code is not None and sl_code is not None and seq_lens.shape[0] == requests and block_size > 0
+    assert bt_code is not None and sl_code is not None and seq_lens.shape[0] == requests
+    assert 0 < block_size < 2**31  # the library takes it as a C int
     return device, requests, width, bt_code, sl_code
 
 

@@ -1151,7 +1151,7 @@ int run_diff(const AttnCall& a, const DiffExtra& x) {
       (x.norm_w != nullptr && !valid_float_dtype(x.norm_dtype)))
     return INT8KV_E_BAD_DTYPE;
   if (x.norm_w != nullptr && !(x.norm_eps > 0.f)) return INT8KV_E_BAD_SHAPE;
-  if (a.D > kDiffMaxD) return INT8KV_E_UNSUPPORTED;
+  if (a.D > kDiffMaxD || a.Hq > 65535) return INT8KV_E_UNSUPPORTED;  // the join numbers the query pairs in grid y
   if (a.B == 0) return INT8KV_OK;
   if (!a.query || !a.kc || !a.vc || !a.bt || !a.sl || !a.q_st || !a.kc_st || !a.vc_st || !a.bt_st || !a.out || !a.o_st || !x.lam)
     return INT8KV_E_NULLPTR;

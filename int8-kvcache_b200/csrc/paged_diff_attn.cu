@@ -186,16 +186,18 @@ template <int NB>
 __device__ __forceinline__ int col_pair(int c) { return NB == 1 ? c & 3 : c; }
 
 // Running softmax of the columns of one block: reference m of columns 2t (index 0) and 2t+1, in log2 units.  It is a score
-// that was the column's maximum when it was set, and follows the maximum only when that has moved more than kSlack above
-// it: probabilities reach up to 2^kSlack, which fp16, bf16 and the fp32 sums hold with the same relative precision as
-// values up to 1.  A step then needs no reduction across the token lanes, just a vote, and the accumulators are rescaled a
-// few times per part instead of in every other tile (32 x 32k tokens, groups of eight: 324 -> 309 us).
-constexpr float kSlack = 8.f;
+// that was the column's maximum when it was set, and follows the maximum only when that has moved more than SLACK above
+// it: probabilities reach up to 2^SLACK, which the 16-bit P and the fp32 sums hold with the same relative precision as
+// values up to 1.  A step then needs no reduction across the token lanes, just a vote, and with SLACK = 8 the accumulators
+// are rescaled a few times per part instead of in every other tile (INT8, 32 x 32k tokens, groups of eight: 324 -> 309
+// us).  SLACK = 0 keeps the largest probability at 1, which is exact however few bits P has: of use where P has the 8 bits
+// of bf16 (8 x 4096 tokens: error against 64 bits 0.0019 of the output's norm instead of 0.0023, of which the output's own
+// rounding is 0.0017; 22.1 us instead of 21.8).
 
 // One online-softmax step over NV / 2 score rows per lane and NB column blocks at once.  x: scores before the factors
 // sc, x[nb][2k] and x[nb][2k+1] being columns 2t and 2t+1 of token row g + 8k, of which the first `valid` count.  x becomes
 // the probabilities 2^(x sc - m); returns whether m moved, and with it the accumulators, by f[nb][0], f[nb][1].
-template <int NB, int NV>
+template <int SLACK, int NB, int NV>
 __device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][NV], const float (&sc)[NB][2], float (&f)[NB][2],
                                              int valid, int g) {
   float y[NB][NV];
@@ -216,7 +218,7 @@ __device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][N
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int k = 0; k < NV; ++k) top = fmaxf(top, y[nb][k]);
-  const bool moved = __any_sync(kFull, top > kSlack);  // also while m is -inf: y is +inf then
+  const bool moved = __any_sync(kFull, top > static_cast<float>(SLACK));  // also while m is -inf: y is +inf then
   if (moved) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -665,7 +667,7 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[nb][4 * u + r] = static_cast<float>(raw[nb][r]);
     }
-    if (softmax_step<NB, 4 * TRIP>(m, x, sc, f, limit - i * kTile, g)) {
+    if (softmax_step<8>(m, x, sc, f, limit - i * kTile, g)) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         sum[nb][0] *= f[nb][0]; sum[nb][1] *= f[nb][1];
@@ -817,7 +819,7 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
       for (int r = 0; r < 4; ++r)  // NB = 1: both K heads met all columns, each column keeps its own map's score
         x[nb][r] = NB == 1 ? (t < 2 ? sm[0][0][r] + sm[0][1][r] : sm[1][0][r] + sm[1][1][r]) : sm[nb][0][r] + sm[nb][1][r];
-    if (softmax_step<NB, 4>(m, x, sc, f, nvalid, g)) {
+    if (softmax_step<0>(m, x, sc, f, nvalid, g)) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         sum[nb][0] *= f[nb][0]; sum[nb][1] *= f[nb][1];
@@ -1100,7 +1102,6 @@ int launch_diff_tiled(const DiffParams& d, const CUtensorMap& tmK, const CUtenso
 
 int launch_diff_merge(const DiffParams& d, cudaStream_t stream) {
   const AttnParams& p = d.a;
-  if (d.heads > 65535) return INT8KV_E_UNSUPPORTED;  // grid y
   const int batch = std::min(kMergeBatch, p.num_splits);
   if (!raise_smem<diff_merge_kernel>(kMergeBatch * 8 * (2 * kDiffMaxD + 4))) return INT8KV_E_LAUNCH;
   const unsigned warps = static_cast<unsigned>((p.D + 31) / 32);  // at most 16

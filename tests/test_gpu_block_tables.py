@@ -161,7 +161,7 @@ def test_refusals(kv):
     free = torch.zeros(4, dtype=torch.int32, device=DEV)
     build = lambda t=bt, s=lens, n=lens, f=free, c=one, bs=16, tok=4, **kw: kv.build_block_tables(t, s, n, f, c, bs, num_tokens=tok, **kw)
     build()
-    for bad in (dict(t=bt.float()), dict(t=bt[0]), dict(s=lens[:1]), dict(s=lens.float()), dict(n=lens.cpu()), dict(bs=0),
+    for bad in (dict(t=bt.float()), dict(t=bt[0]), dict(s=lens[:1]), dict(s=lens.float()), dict(n=lens.cpu()), dict(bs=0), dict(bs=2**32 + 16),
                 dict(f=free.float()), dict(c=one.int()), dict(c=torch.zeros(2, dtype=torch.int64, device=DEV)), dict(tok=-1),
                 dict(tok=2**31), dict(t=torch.zeros(1, 4, dtype=torch.int32, device=DEV).expand(2, 4)), dict(f=free.cpu())):
         with pytest.raises(AssertionError):
