@@ -173,14 +173,60 @@ __device__ __forceinline__ uint32_t tab_moves(const TableParams& p, const TabTot
 }
 
 // The write phase of warp `me` of `warps`: a run of consecutive tokens, then one of blocks that move.  The warp finds the
-// requests of the run's first and last item together.  Mostly they are the same (a prompt): then everything but the
-// position is uniform.  Otherwise each lane searches between them, five steps where every token is another
-// request's.
+// requests of the run's first and last item together.  Runs of few requests (prompts) go request by request, with
+// everything but the position uniform; in the others each lane searches between the two, five steps where every token is
+// another request's.
 __device__ __forceinline__ void tab_run(uint32_t items, uint32_t me, uint32_t warps, uint32_t& lo, uint32_t& hi) {
   const uint32_t rows = (items >> 5) + 1, per = (rows + warps - 1) / warps;  // rows of 32 items, per warp
   const uint64_t a = static_cast<uint64_t>(me) * per * 32u, b = a + per * 32ull;
   lo = static_cast<uint32_t>(a < items ? a : items);
   hi = static_cast<uint32_t>(b < items ? b : items);
+}
+
+// Slots of tokens lo + lane, lo + lane + 32, ... below hi, at positions p0 + token, through block ids ids[j * stride] of
+// logical blocks j < blocks: four loads in flight per lane.
+template <typename T>
+__device__ __forceinline__ void tab_span(int64_t* slots, uint32_t lo, uint32_t hi, uint32_t p0, int S, int shift, const T* ids,
+                                         int64_t stride, uint32_t blocks, int lane) {
+  constexpr int kAhead = 4;
+  for (uint32_t tok = lo + lane; tok < hi; tok += kAhead * kWarp) {
+    int64_t blk[kAhead];
+    uint32_t off[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t pos = p0 + tok + u * kWarp;
+      const uint32_t j = shift >= 0 ? pos >> shift : pos / static_cast<uint32_t>(S);
+      off[u] = pos - j * S;
+      blk[u] = tok + u * kWarp < hi && j < blocks ? static_cast<int64_t>(ids[j * stride]) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (tok + u * kWarp < hi) slots[tok + u * kWarp] = blk[u] < 0 ? -1 : blk[u] * S + off[u];
+  }
+}
+
+// Slots of tokens [lo, hi) of the packed order, all of request b, by one warp.
+__device__ __forceinline__ void tab_request_slots(const TableParams& p, const TabRecord* rec, const TabTotals& tot, int b,
+                                                  uint32_t lo, uint32_t hi, int lane) {
+  const TabRecord r = rec[b];
+  if (r.cached < 0 || r.cached + hi > 0x7fffffffll) {  // refused, or positions beyond 31 bits
+    for (uint32_t tok = lo + lane; tok < hi; tok += kWarp) p.slots[tok] = tab_slot(p, rec, tot, b, tok);
+    return;
+  }
+  const uint32_t p0 = static_cast<uint32_t>(r.cached) - r.start;
+  uint32_t known = hi;  // tokens below this one lie in blocks that the table has
+  if (p.mode == kTabGrow) {
+    const uint32_t left = static_cast<uint32_t>(r.cached) % static_cast<uint32_t>(p.block_size);
+    known = left == 0u ? r.start : r.start + (p.block_size - left);
+    known = max(lo, min(hi, known));
+  }
+  const uint32_t width = static_cast<uint32_t>(p.width);
+  auto span = [&](uint32_t from, uint32_t to, const void* ids, int is_i64, int64_t first, int64_t stride, uint32_t blocks) {
+    if (is_i64) tab_span(p.slots, from, to, p0, p.block_size, p.block_shift, static_cast<const int64_t*>(ids) + first, stride, blocks, lane);
+    else tab_span(p.slots, from, to, p0, p.block_size, p.block_shift, static_cast<const int32_t*>(ids) + first, stride, blocks, lane);
+  };
+  if (lo < known) span(lo, known, p.bt, p.bt_is_i64, b * p.bt_st[0], p.bt_st[1], width);
+  if (known < hi) span(known, hi, p.free_blocks, p.free_is_i64, tot.cursor + r.shift, 1, width);
 }
 
 __device__ __forceinline__ void tab_write_slots(const TableParams& p, const TabRecord* rec, const TabTotals& tot, uint32_t me,
@@ -191,22 +237,8 @@ __device__ __forceinline__ void tab_write_slots(const TableParams& p, const TabR
   if (lo < live) {
     const int b0 = tab_owner_warp<true>(rec, p.R, lo, lane);
     const int b1 = tab_owner_warp<true>(rec, p.R, live - 1, lane);
-    const TabRecord r = rec[b0];
-    if (b0 == b1 && r.cached >= 0 && r.cached + (live - r.start) <= 0xffffffffll && p.width <= 0x7fffffffll) {
-      const uint32_t S = p.block_size, cached = static_cast<uint32_t>(r.cached), p0 = cached - r.start;
-      const bool grow = p.mode == kTabGrow;
-      const uint32_t width = static_cast<uint32_t>(p.width);
-      const int64_t row = b0 * p.bt_st[0], list = tot.cursor + r.shift;
-#pragma unroll 4
-      for (uint32_t tok = lo + lane; tok < live; tok += kWarp) {
-        const uint32_t pos = p0 + tok;
-        const uint32_t j = p.block_shift >= 0 ? pos >> p.block_shift : pos / S;
-        const uint32_t begin = j * S;
-        int64_t blk = -1;
-        if (grow && begin >= cached) blk = load_index(p.free_blocks, p.free_is_i64, list + j);
-        else if (j < width) blk = load_index_rw(p.bt, p.bt_is_i64, row + j * p.bt_st[1]);
-        p.slots[tok] = blk < 0 ? -1 : blk * S + (pos - begin);
-      }
+    if (static_cast<uint32_t>(b1 - b0) <= (live - lo) / kWarp) {
+      for (int b = b0; b <= b1; ++b) tab_request_slots(p, rec, tot, b, max(lo, rec[b].start), b < b1 ? min(live, rec[b + 1].start) : live, lane);
     } else {
       for (uint32_t tok = lo + lane; tok < live; tok += kWarp)
         p.slots[tok] = tab_slot(p, rec, tot, tab_owner<true>(rec, b0, b1 + 1, tok), tok);
@@ -222,7 +254,6 @@ __device__ __forceinline__ void tab_write_moves(const TableParams& p, const TabR
   if (lo >= hi) return;
   const int b0 = tab_owner_warp<false>(rec, p.R, lo, lane);
   const int b1 = tab_owner_warp<false>(rec, p.R, hi - 1, lane);
-#pragma unroll 4
   for (uint32_t k = lo + lane; k < hi; k += kWarp)
     tab_move(p, rec, tot, b0 == b1 ? b0 : tab_owner<false>(rec, b0, b1 + 1, k), k);
 }
