@@ -43,6 +43,7 @@ extern "C" {
 #define INT8KV_BF16 0
 #define INT8KV_FP16 1
 #define INT8KV_FP32 2
+#define INT8KV_INT8 3 /* caches only (int8kv_diff_args) */
 
 /* Bits set by a kernel in the workspace's trailing status word (see int8kv_workspace_status_offset). */
 #define INT8KV_DEV_WAIT_TIMEOUT 1u /* a bounded wait for a staged page ran out; result invalid */
@@ -337,42 +338,38 @@ int int8kv_static_ws_address(void** device_ptr);
  *   out = out_scale * o                                                      without norm_weight
  *   out = out_scale * norm_weight * o / sqrt(mean(o^2) + norm_eps)           with it (mean over the 2 D values)
  * A sequence with seq_len <= 0 yields zeros.  D <= 256.
- *   k_scale / v_scale  [2 * num_kv_pairs] fp32 (int8 form): the scales the cache was written with
- *   lam                [num_heads] or, with lam_stride 0, one value; lam_dtype and norm_dtype are float dtype codes
- *   norm_weight        [2 D] contiguous, or NULL; norm_eps > 0 with it
- *   num_splits         0 = choose from the shape, >= 1 = exactly that many (at most int8kv_max_splits())
- *   workspace          int8kv_diff_workspace_bytes() bytes, 16-byte aligned (always needed: the maps' rows go through it)
- *   status             device word for INT8KV_DEV_* bits, or NULL
+ * Every member of the argument block is 8 bytes wide, so that a binding can fill it as one flat record.
  */
+typedef struct int8kv_diff_args {
+  const void* query;         /* [batch, 2 * num_heads, head_dim] */
+  const void* key_cache;     /* [num_blocks, block_size, 2 * num_kv_pairs, head_dim] */
+  const void* value_cache;
+  const void* block_tables;  /* [batch, bt_width] */
+  const void* seq_lens;      /* [batch] */
+  const float* k_scale;      /* [2 * num_kv_pairs], the scales an INT8 cache was written with; NULL for float caches */
+  const float* v_scale;
+  const void* lam;           /* [num_heads] or, with lam_stride 0, one value */
+  const void* norm_weight;   /* [2 * head_dim] contiguous, or NULL: no norm */
+  void* out;                 /* [batch, num_heads, 2 * head_dim] */
+  void* workspace;           /* int8kv_diff_workspace_bytes() bytes, 16-byte aligned: the parts' rows go through it */
+  unsigned int* status;      /* device word for INT8KV_DEV_* bits, or NULL */
+  void* stream;
+  int64_t q_strides[3], key_cache_strides[4], value_cache_strides[4], bt_strides[2], out_strides[3];
+  int64_t lam_stride;
+  int64_t batch, num_heads, num_kv_pairs, head_dim, num_blocks, block_size, bt_width;
+  int64_t max_seq_len_hint;  /* upper bound of seq_lens used only to size the grid; <= 0 means bt_width * block_size */
+  int64_t num_splits;        /* 0 = choose from the shape, >= 1 = that many (at most int8kv_max_splits()) */
+  int64_t workspace_bytes;
+  int64_t q_dtype, cache_dtype, lam_dtype, norm_dtype, out_dtype; /* cache_dtype: INT8KV_INT8, INT8KV_BF16, INT8KV_FP16 */
+  int64_t bt_is_i64, sl_is_i64;
+  double norm_eps;           /* > 0 with a norm_weight */
+  double out_scale;
+} int8kv_diff_args;
+
 int64_t int8kv_diff_workspace_bytes(int batch, int num_heads, int num_kv_pairs, int head_dim, int64_t max_seq_len,
                                     int block_size, int num_splits, int sm_count);
 
-int int8kv_paged_diff_attn_int8(const void* query, int q_dtype, const int64_t q_strides[3],
-                                int batch, int num_heads, int num_kv_pairs, int head_dim,
-                                const int8_t* key_cache, const int8_t* value_cache,
-                                const int64_t key_cache_strides[4], const int64_t value_cache_strides[4],
-                                int64_t num_blocks, int block_size,
-                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
-                                const void* seq_lens, int sl_is_i64, int64_t max_seq_len_hint,
-                                const float* k_scale, const float* v_scale,
-                                const void* lam, int lam_dtype, int64_t lam_stride,
-                                const void* norm_weight, int norm_dtype, float norm_eps, float out_scale,
-                                void* out, int out_dtype, const int64_t out_strides[3],
-                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
-                                void* stream);
-
-int int8kv_paged_diff_attn_bf16(const void* query, int q_dtype, const int64_t q_strides[3],
-                                int batch, int num_heads, int num_kv_pairs, int head_dim,
-                                const void* key_cache, const void* value_cache, int cache_dtype,
-                                const int64_t key_cache_strides[4], const int64_t value_cache_strides[4],
-                                int64_t num_blocks, int block_size,
-                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
-                                const void* seq_lens, int sl_is_i64, int64_t max_seq_len_hint,
-                                const void* lam, int lam_dtype, int64_t lam_stride,
-                                const void* norm_weight, int norm_dtype, float norm_eps, float out_scale,
-                                void* out, int out_dtype, const int64_t out_strides[3],
-                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
-                                void* stream);
+int int8kv_paged_diff_attn(const int8kv_diff_args* args);
 
 /*
  * Block tables and slot maps from request lengths, on the device (no counterpart in the reference, whose tests and
@@ -408,26 +405,27 @@ int int8kv_paged_diff_attn_bf16(const void* query, int q_dtype, const int64_t q_
  */
 int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items, int in_place);
 
-int int8kv_build_block_tables(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
-                              int num_requests, int block_size,
-                              void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
-                              const void* free_blocks, int fb_is_i64, int64_t num_free,
-                              const int64_t* free_cursor, int64_t* free_cursor_out, void* seq_lens_out,
-                              int64_t* slot_mapping, int64_t num_tokens, int32_t* query_start,
-                              void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct int8kv_table_args { /* every member 8 bytes wide, as in int8kv_diff_args */
+  const void* seq_lens;        /* [num_requests] */
+  const void* new_lens;        /* [num_requests] (not for a release) */
+  const uint8_t* finished;     /* [num_requests] (release) */
+  void* block_tables;          /* [num_requests, bt_width]; written by int8kv_build_block_tables only */
+  void* free_blocks;           /* [num_free] (build: read, release: written) */
+  const int64_t* free_cursor;  /* [1] (build, release) */
+  int64_t* free_cursor_out;
+  void* seq_lens_out;          /* [num_requests], the type of seq_lens (build, release) */
+  int64_t* slot_mapping;       /* [num_tokens] (not for a release) */
+  int32_t* query_start;        /* [num_requests + 1] (not for a release) */
+  void* workspace;
+  void* stream;
+  int64_t sl_is_i64, nl_is_i64, bt_is_i64, fb_is_i64;
+  int64_t num_requests, block_size, bt_strides[2], bt_width, num_free, num_tokens;
+  int64_t workspace_bytes;
+} int8kv_table_args;
 
-int int8kv_build_slot_mapping(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
-                              int num_requests, int block_size,
-                              const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
-                              int64_t* slot_mapping, int64_t num_tokens, int32_t* query_start,
-                              void* workspace, int64_t workspace_bytes, void* stream);
-
-int int8kv_release_block_tables(const void* seq_lens, int sl_is_i64, const uint8_t* finished,
-                                int num_requests, int block_size,
-                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
-                                void* free_blocks, int fb_is_i64, int64_t num_free,
-                                const int64_t* free_cursor, int64_t* free_cursor_out, void* seq_lens_out,
-                                void* workspace, int64_t workspace_bytes, void* stream);
+int int8kv_build_block_tables(const int8kv_table_args* args);
+int int8kv_build_slot_mapping(const int8kv_table_args* args);
+int int8kv_release_block_tables(const int8kv_table_args* args);
 
 /*
  * Merge `num_parts` partial results.  Replaces _merge_split_kv_kernel (reference

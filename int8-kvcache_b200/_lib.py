@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -27,7 +28,7 @@ SPLITS_AUTO, SPLITS_PLANNED = 0, -1
 FLAG_QUANTIZE_Q, FLAG_INPUTS_READY = 1, 2
 PLAN_HEADER_TAG = 0x504C414E
 
-BF16, FP16, FP32 = 0, 1, 2
+BF16, FP16, FP32, INT8 = 0, 1, 2, 3
 
 _I64P = C.POINTER(C.c_int64)
 _VP = C.c_void_p
@@ -50,6 +51,11 @@ class Exchange(C.Structure):
 
     _fields_ = [("world", C.c_int), ("rank", C.c_int), ("peer_buffers", _VP * 16), ("buffer_bytes", C.c_int64)]
 
+
+# int8kv_diff_args and int8kv_table_args of include/int8kv_b200.h as flat records of 8-byte members.  Such an argument block
+# is packed by one call in C, where an argument list pays a conversion per argument (47 arguments: about 4 us).
+DIFF_ARGS = struct.Struct("=13Q16q18q2d")
+TABLE_ARGS = struct.Struct("=12Q12q")
 
 _SIGNATURES = {
     "int8kv_abi_version": (C.c_int, []),
@@ -124,34 +130,11 @@ _SIGNATURES = {
     "int8kv_diff_workspace_bytes": (
         C.c_int64, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int],
     ),
-    "int8kv_paged_diff_attn_int8": (
-        C.c_int,
-        [_VP, C.c_int, _I64P, C.c_int, C.c_int, C.c_int, C.c_int, _VP, _VP, _I64P, _I64P, C.c_int64, C.c_int,
-         _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64, _VP, _VP, _VP, C.c_int, C.c_int64,
-         _VP, C.c_int, C.c_float, C.c_float, _VP, C.c_int, _I64P, C.c_int, _VP, C.c_int64, _VP, _VP],
-    ),
-    "int8kv_paged_diff_attn_bf16": (
-        C.c_int,
-        [_VP, C.c_int, _I64P, C.c_int, C.c_int, C.c_int, C.c_int, _VP, _VP, C.c_int, _I64P, _I64P, C.c_int64, C.c_int,
-         _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64, _VP, C.c_int, C.c_int64,
-         _VP, C.c_int, C.c_float, C.c_float, _VP, C.c_int, _I64P, C.c_int, _VP, C.c_int64, _VP, _VP],
-    ),
+    "int8kv_paged_diff_attn": (C.c_int, [C.c_char_p]),
     "int8kv_block_tables_workspace_bytes": (C.c_int64, [C.c_int, C.c_int64, C.c_int]),
-    "int8kv_build_block_tables": (
-        C.c_int,
-        [_VP, C.c_int, _VP, C.c_int, C.c_int, C.c_int, _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64,
-         _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP, C.c_int64, _VP],
-    ),
-    "int8kv_build_slot_mapping": (
-        C.c_int,
-        [_VP, C.c_int, _VP, C.c_int, C.c_int, C.c_int, _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int64, _VP,
-         _VP, C.c_int64, _VP],
-    ),
-    "int8kv_release_block_tables": (
-        C.c_int,
-        [_VP, C.c_int, _VP, C.c_int, C.c_int, _VP, C.c_int, _I64P, C.c_int64, _VP, C.c_int, C.c_int64,
-         _VP, _VP, _VP, _VP, C.c_int64, _VP],
-    ),
+    "int8kv_build_block_tables": (C.c_int, [C.c_char_p]),
+    "int8kv_build_slot_mapping": (C.c_int, [C.c_char_p]),
+    "int8kv_release_block_tables": (C.c_int, [C.c_char_p]),
     "int8kv_static_ws_status": (C.c_int, [_VP, C.c_int, _VP]),
     "int8kv_static_ws_address": (C.c_int, [C.POINTER(_VP)]),
     "int8kv_exchange_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int, C.c_int]),

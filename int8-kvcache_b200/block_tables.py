@@ -20,7 +20,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _call, _require_lib
+from .ops import _call, _require_lib, _stream_ptr
 
 _INDEX_CODES = {torch.int32: 0, torch.int64: 1}
 _MAX_TOKENS = 2**31 - 1
@@ -112,14 +112,10 @@ def build_block_tables(
     cursor_ptr, cursor_out = free_cursor.data_ptr(), out.free_cursor.data_ptr()
     in_place = lens_out == lens_ptr or lens_out == new_ptr or cursor_ptr == cursor_out
     ws, ws_ptr, ws_bytes = _workspace(R, num_tokens + num_tokens // block_size + R, in_place, device)
-    rc = _call(
-        device, lib.int8kv_build_block_tables,
-        lens_ptr, sl_code, new_ptr, nl_code, R, block_size,
-        block_tables.data_ptr(), bt_code, _lib.i64(bt_st), width,
-        free_blocks.data_ptr(), fb_code, free_blocks.shape[0],
-        cursor_ptr, cursor_out, lens_out,
-        out.slot_mapping.data_ptr(), num_tokens, out.query_start.data_ptr(), ws_ptr, ws_bytes,
-    )
+    rc = _call(device, lib.int8kv_build_block_tables, _lib.TABLE_ARGS.pack(
+        lens_ptr, new_ptr, 0, block_tables.data_ptr(), free_blocks.data_ptr(), cursor_ptr, cursor_out, lens_out,
+        out.slot_mapping.data_ptr(), out.query_start.data_ptr(), ws_ptr, _stream_ptr(device),
+        sl_code, nl_code, bt_code, fb_code, R, block_size, *bt_st, width, free_blocks.shape[0], num_tokens, ws_bytes))
     if rc != _lib.OK:
         _lib.check("int8kv_build_block_tables", rc)
     return out
@@ -150,12 +146,10 @@ def build_slot_mapping(
     lib = _require_lib()
     seq_lens, new_lens = seq_lens.contiguous(), new_lens.contiguous()
     ws, ws_ptr, ws_bytes = _workspace(R, num_tokens, False, device)
-    rc = _call(
-        device, lib.int8kv_build_slot_mapping,
-        seq_lens.data_ptr(), sl_code, new_lens.data_ptr(), nl_code, R, block_size,
-        block_tables.data_ptr(), bt_code, _lib.i64(block_tables.stride()), width,
-        out[0].data_ptr(), num_tokens, out[1].data_ptr(), ws_ptr, ws_bytes,
-    )
+    rc = _call(device, lib.int8kv_build_slot_mapping, _lib.TABLE_ARGS.pack(
+        seq_lens.data_ptr(), new_lens.data_ptr(), 0, block_tables.data_ptr(), 0, 0, 0, 0,
+        out[0].data_ptr(), out[1].data_ptr(), ws_ptr, _stream_ptr(device),
+        sl_code, nl_code, bt_code, 0, R, block_size, *block_tables.stride(), width, 0, num_tokens, ws_bytes))
     if rc != _lib.OK:
         _lib.check("int8kv_build_slot_mapping", rc)
     return out
@@ -190,13 +184,10 @@ def release_block_tables(
     lens_ptr, lens_out, cursor_ptr, cursor_out = (
         seq_lens.data_ptr(), out[0].data_ptr(), free_cursor.data_ptr(), out[1].data_ptr())
     ws, ws_ptr, ws_bytes = _workspace(R, min(R * width, N), lens_ptr == lens_out or cursor_ptr == cursor_out, device)
-    rc = _call(
-        device, lib.int8kv_release_block_tables,
-        lens_ptr, sl_code, finished.data_ptr(), R, block_size,
-        block_tables.data_ptr(), bt_code, _lib.i64(block_tables.stride()), width,
-        free_blocks.data_ptr(), fb_code, N,
-        cursor_ptr, cursor_out, lens_out, ws_ptr, ws_bytes,
-    )
+    rc = _call(device, lib.int8kv_release_block_tables, _lib.TABLE_ARGS.pack(
+        lens_ptr, 0, finished.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(), cursor_ptr, cursor_out, lens_out,
+        0, 0, ws_ptr, _stream_ptr(device),
+        sl_code, 0, bt_code, fb_code, R, block_size, *block_tables.stride(), width, N, 0, ws_bytes))
     if rc != _lib.OK:
         _lib.check("int8kv_release_block_tables", rc)
     return out

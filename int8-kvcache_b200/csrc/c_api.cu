@@ -998,23 +998,42 @@ namespace {
 constexpr int64_t kMaxIndex = (int64_t(1) << 31) - 1;  // tokens, columns and list entries are numbered in 32 bits
 
 // The arguments that the three operators share.
-int table_params(TableParams& p, int mode, const void* lens, int lens_is_i64, int R, int block_size, void* bt,
-                 int bt_is_i64, const int64_t* bt_st, int64_t width) {
+int table_params(TableParams& p, int mode, const int8kv_table_args* a) {
   std::memset(&p, 0, sizeof(p));
-  if (R < 0 || R >= kMaxIndex || block_size <= 0 || width < 0 || width >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
-  if (R > 0 && (!lens || !bt_st || (width > 0 && !bt))) return INT8KV_E_NULLPTR;
+  if (a == nullptr) return INT8KV_E_NULLPTR;
+  if (a->num_requests < 0 || a->num_requests >= kMaxIndex || a->block_size <= 0 || a->block_size >= kMaxIndex ||
+      a->bt_width < 0 || a->bt_width >= kMaxIndex)
+    return INT8KV_E_BAD_SHAPE;
+  if (a->num_requests > 0 && (!a->seq_lens || (a->bt_width > 0 && !a->block_tables))) return INT8KV_E_NULLPTR;
   p.mode = mode;
-  p.R = R; p.block_size = block_size; p.width = width;
-  p.bt = bt; p.bt_is_i64 = bt_is_i64;
-  if (bt_st) { p.bt_st[0] = bt_st[0]; p.bt_st[1] = bt_st[1]; }
-  p.lens = lens; p.lens_is_i64 = lens_is_i64;
+  p.R = static_cast<int>(a->num_requests); p.block_size = static_cast<int>(a->block_size); p.width = a->bt_width;
+  p.bt = a->block_tables; p.bt_is_i64 = a->bt_is_i64 != 0; p.bt_st[0] = a->bt_strides[0]; p.bt_st[1] = a->bt_strides[1];
+  p.lens = a->seq_lens; p.lens_is_i64 = a->sl_is_i64 != 0;
+  if (mode != kTabRelease) {
+    if (a->num_tokens < 0 || a->num_tokens >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
+    if (!a->query_start || (p.R > 0 && !a->new_lens) || (a->num_tokens > 0 && !a->slot_mapping)) return INT8KV_E_NULLPTR;
+    p.new_lens = a->new_lens; p.new_is_i64 = a->nl_is_i64 != 0;
+    p.slots = a->slot_mapping; p.num_tokens = a->num_tokens; p.query_start = a->query_start;
+  }
+  if (mode == kTabRelease) {
+    if (p.R > 0 && !a->finished) return INT8KV_E_NULLPTR;
+    p.finished = a->finished;
+  }
+  if (mode != kTabSlots) {
+    if (a->num_free < 0 || a->num_free >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
+    if (!a->free_cursor || !a->free_cursor_out || (a->num_free > 0 && !a->free_blocks) || (p.R > 0 && !a->seq_lens_out))
+      return INT8KV_E_NULLPTR;
+    p.free_blocks = a->free_blocks; p.free_out = a->free_blocks; p.free_is_i64 = a->fb_is_i64 != 0; p.num_free = a->num_free;
+    p.cursor = a->free_cursor; p.cursor_out = a->free_cursor_out; p.lens_out = a->seq_lens_out;
+  }
   return INT8KV_OK;
 }
 
-int run_tables(const TableParams& p, int64_t items, void* ws, int64_t ws_size, void* stream) {
+int run_tables(const TableParams& p, int64_t items, const int8kv_table_args* a) {
   const int64_t need = table_single_launch(p, items) ? 0 : table_workspace_bytes(p.R);
-  if (need > 0 && (ws == nullptr || ws_size < need || (reinterpret_cast<uintptr_t>(ws) & 15u))) return INT8KV_E_WORKSPACE;
-  return launch_tables(p, ws, items, device_sm_count(), static_cast<cudaStream_t>(stream));
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15u)))
+    return INT8KV_E_WORKSPACE;
+  return launch_tables(p, a->workspace, items, device_sm_count(), static_cast<cudaStream_t>(a->stream));
 }
 
 }  // namespace
@@ -1034,59 +1053,22 @@ int64_t int8kv_block_tables_workspace_bytes(int num_requests, int64_t items, int
   return table_single_launch(p, items) ? 0 : table_workspace_bytes(num_requests);
 }
 
-int int8kv_build_block_tables(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
-                              int num_requests, int block_size, void* block_tables, int bt_is_i64,
-                              const int64_t bt_strides[2], int64_t bt_width, const void* free_blocks, int fb_is_i64,
-                              int64_t num_free, const int64_t* free_cursor, int64_t* free_cursor_out,
-                              void* seq_lens_out, int64_t* slot_mapping, int64_t num_tokens, int32_t* query_start,
-                              void* workspace, int64_t workspace_bytes, void* stream) {
+int int8kv_build_block_tables(const int8kv_table_args* args) {
   TableParams p;
-  const int rc = table_params(p, kTabGrow, seq_lens, sl_is_i64, num_requests, block_size, block_tables, bt_is_i64,
-                              bt_strides, bt_width);
-  if (rc != INT8KV_OK) return rc;
-  if (num_free < 0 || num_free >= kMaxIndex || num_tokens < 0 || num_tokens >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
-  if (!free_cursor || !free_cursor_out || !query_start) return INT8KV_E_NULLPTR;
-  if ((num_requests > 0 && (!new_lens || !seq_lens_out)) || (num_free > 0 && !free_blocks) ||
-      (num_tokens > 0 && !slot_mapping))
-    return INT8KV_E_NULLPTR;
-  p.new_lens = new_lens; p.new_is_i64 = nl_is_i64; p.lens_out = seq_lens_out;
-  p.free_blocks = free_blocks; p.free_is_i64 = fb_is_i64; p.num_free = num_free;
-  p.cursor = free_cursor; p.cursor_out = free_cursor_out;
-  p.slots = slot_mapping; p.num_tokens = num_tokens; p.query_start = query_start;
-  return run_tables(p, num_tokens + num_tokens / block_size + num_requests, workspace, workspace_bytes, stream);
+  const int rc = table_params(p, kTabGrow, args);
+  return rc != INT8KV_OK ? rc : run_tables(p, p.num_tokens + p.num_tokens / p.block_size + p.R, args);
 }
 
-int int8kv_build_slot_mapping(const void* seq_lens, int sl_is_i64, const void* new_lens, int nl_is_i64,
-                              int num_requests, int block_size, const void* block_tables, int bt_is_i64,
-                              const int64_t bt_strides[2], int64_t bt_width, int64_t* slot_mapping, int64_t num_tokens,
-                              int32_t* query_start, void* workspace, int64_t workspace_bytes, void* stream) {
+int int8kv_build_slot_mapping(const int8kv_table_args* args) {
   TableParams p;
-  const int rc = table_params(p, kTabSlots, seq_lens, sl_is_i64, num_requests, block_size,
-                              const_cast<void*>(block_tables), bt_is_i64, bt_strides, bt_width);
-  if (rc != INT8KV_OK) return rc;
-  if (num_tokens < 0 || num_tokens >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
-  if (!query_start || (num_requests > 0 && !new_lens) || (num_tokens > 0 && !slot_mapping)) return INT8KV_E_NULLPTR;
-  p.new_lens = new_lens; p.new_is_i64 = nl_is_i64;
-  p.slots = slot_mapping; p.num_tokens = num_tokens; p.query_start = query_start;
-  return run_tables(p, num_tokens, workspace, workspace_bytes, stream);
+  const int rc = table_params(p, kTabSlots, args);
+  return rc != INT8KV_OK ? rc : run_tables(p, p.num_tokens, args);
 }
 
-int int8kv_release_block_tables(const void* seq_lens, int sl_is_i64, const uint8_t* finished, int num_requests,
-                                int block_size, const void* block_tables, int bt_is_i64, const int64_t bt_strides[2],
-                                int64_t bt_width, void* free_blocks, int fb_is_i64, int64_t num_free,
-                                const int64_t* free_cursor, int64_t* free_cursor_out, void* seq_lens_out,
-                                void* workspace, int64_t workspace_bytes, void* stream) {
+int int8kv_release_block_tables(const int8kv_table_args* args) {
   TableParams p;
-  const int rc = table_params(p, kTabRelease, seq_lens, sl_is_i64, num_requests, block_size,
-                              const_cast<void*>(block_tables), bt_is_i64, bt_strides, bt_width);
-  if (rc != INT8KV_OK) return rc;
-  if (num_free < 0 || num_free >= kMaxIndex) return INT8KV_E_BAD_SHAPE;
-  if (!free_cursor || !free_cursor_out || (num_free > 0 && !free_blocks)) return INT8KV_E_NULLPTR;
-  if (num_requests > 0 && (!finished || !seq_lens_out)) return INT8KV_E_NULLPTR;
-  p.finished = finished; p.lens_out = seq_lens_out;
-  p.free_out = free_blocks; p.free_is_i64 = fb_is_i64; p.num_free = num_free;
-  p.cursor = free_cursor; p.cursor_out = free_cursor_out;
-  return run_tables(p, std::min<int64_t>(num_requests * bt_width, num_free), workspace, workspace_bytes, stream);
+  const int rc = table_params(p, kTabRelease, args);
+  return rc != INT8KV_OK ? rc : run_tables(p, std::min<int64_t>(p.R * p.width, p.num_free), args);
 }
 
 }  // extern "C"
@@ -1137,79 +1119,82 @@ bool diff_tiled_shape(int D, int group, int block_size) {
   return (D == 64 || D == 128) && group <= 8 && block_size % 16 == 0;
 }
 
-struct DiffExtra {
-  const void* lam; int lam_dtype; int64_t lam_stride;
-  const void* norm_w; int norm_dtype; float norm_eps; float out_scale;
-};
-
-// `a` in the caller's terms: Hq = query pairs, Hkv = KV pairs, D = head dim.
-int run_diff(const AttnCall& a, const DiffExtra& x) {
-  if (a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.D <= 0 || a.block_size <= 0 || a.num_blocks < 0 || a.bt_width < 0)
+int run_diff(const int8kv_diff_args& a) {
+  if (a.batch < 0 || a.num_heads <= 0 || a.num_kv_pairs <= 0 || a.head_dim <= 0 || a.block_size <= 0 || a.num_blocks < 0 ||
+      a.bt_width < 0 || a.batch >= kMaxIndex || a.num_heads >= kMaxIndex || a.block_size >= kMaxIndex || a.bt_width >= kMaxIndex)
     return INT8KV_E_BAD_SHAPE;
-  if (a.Hq % a.Hkv != 0 || a.num_splits < 0 || a.num_splits > kMaxSplits) return INT8KV_E_BAD_SHAPE;
-  if (!valid_float_dtype(a.q_dtype) || !valid_float_dtype(a.out_dtype) || !valid_float_dtype(x.lam_dtype) ||
-      (x.norm_w != nullptr && !valid_float_dtype(x.norm_dtype)))
-    return INT8KV_E_BAD_DTYPE;
-  if (x.norm_w != nullptr && !(x.norm_eps > 0.f)) return INT8KV_E_BAD_SHAPE;
-  if (a.D > kDiffMaxD || a.Hq > 65535) return INT8KV_E_UNSUPPORTED;  // the join numbers the query pairs in grid y
-  if (a.B == 0) return INT8KV_OK;
-  if (!a.query || !a.kc || !a.vc || !a.bt || !a.sl || !a.q_st || !a.kc_st || !a.vc_st || !a.bt_st || !a.out || !a.o_st || !x.lam)
-    return INT8KV_E_NULLPTR;
-  if (a.cache_kind == kCacheInt8 && (!a.k_scale || !a.v_scale)) return INT8KV_E_NULLPTR;
-  if (a.kc_st[3] != 1 || a.vc_st[3] != 1) return INT8KV_E_UNSUPPORTED;
+  if (a.num_heads % a.num_kv_pairs != 0 || a.num_splits < 0 || a.num_splits > kMaxSplits) return INT8KV_E_BAD_SHAPE;
+  const bool norm = a.norm_weight != nullptr;
+  for (const int64_t d : {a.q_dtype, a.out_dtype, a.lam_dtype, norm ? a.norm_dtype : int64_t(INT8KV_FP32)})
+    if (d < 0 || d > INT8KV_FP32) return INT8KV_E_BAD_DTYPE;
+  if (a.cache_dtype != INT8KV_INT8 && a.cache_dtype != INT8KV_BF16 && a.cache_dtype != INT8KV_FP16) return INT8KV_E_BAD_DTYPE;
+  if (norm && !(a.norm_eps > 0.0)) return INT8KV_E_BAD_SHAPE;
+  if (a.head_dim > kDiffMaxD || a.num_heads > 65535) return INT8KV_E_UNSUPPORTED;  // the join numbers the query pairs in grid y
+  if (a.batch == 0) return INT8KV_OK;
+  if (!a.query || !a.key_cache || !a.value_cache || !a.block_tables || !a.seq_lens || !a.out || !a.lam) return INT8KV_E_NULLPTR;
+  const bool int8_cache = a.cache_dtype == INT8KV_INT8;
+  if (int8_cache && (!a.k_scale || !a.v_scale)) return INT8KV_E_NULLPTR;
+  if (a.key_cache_strides[3] != 1 || a.value_cache_strides[3] != 1) return INT8KV_E_UNSUPPORTED;
 
+  const int kind = int8_cache ? kCacheInt8 : (a.cache_dtype == INT8KV_BF16 ? kCacheBf16 : kCacheFp16);
+  const int B = static_cast<int>(a.batch), heads = static_cast<int>(a.num_heads), pairs = static_cast<int>(a.num_kv_pairs);
+  const int D = static_cast<int>(a.head_dim), block_size = static_cast<int>(a.block_size);
   const int sm = device_sm_count();
   const int64_t cap = a.bt_width * a.block_size;
-  const int64_t max_seq = a.max_seq_hint > 0 ? std::min(a.max_seq_hint, cap) : cap;
+  const int64_t max_seq = a.max_seq_len_hint > 0 ? std::min(a.max_seq_len_hint, cap) : cap;
   const int64_t tiles = (max_seq + 15) / 16;
-  const bool int8_cache = a.cache_kind == kCacheInt8;
   const int esz = int8_cache ? 1 : 2;
   // INT8 rows of 64 values: the two heads of a pair are staged as one row, so they have to be neighbours
-  const bool pair_rows = int8_cache && a.D == 64;
-  const bool tiled = diff_tiled_shape(a.D, a.Hq / a.Hkv, a.block_size) && tma_friendly(a.kc, esz, a.kc_st, a.num_blocks) &&
-                     tma_friendly(a.vc, esz, a.vc_st, a.num_blocks) && (!pair_rows || (a.kc_st[2] == 64 && a.vc_st[2] == 64));
-  const int S = diff_parts(tiled, a.cache_kind, a.B, a.Hq, a.Hkv, a.D, max_seq, a.num_splits, sm);
-  if (a.ws == nullptr || (reinterpret_cast<uintptr_t>(a.ws) & 15u) ||
-      a.ws_bytes < diff_rows_bytes(static_cast<int64_t>(S) * a.B * 2 * a.Hq, a.D))
+  const bool pair_rows = int8_cache && D == 64;
+  const bool tiled = diff_tiled_shape(D, heads / pairs, block_size) && tma_friendly(a.key_cache, esz, a.key_cache_strides, a.num_blocks) &&
+                     tma_friendly(a.value_cache, esz, a.value_cache_strides, a.num_blocks) &&
+                     (!pair_rows || (a.key_cache_strides[2] == 64 && a.value_cache_strides[2] == 64));
+  const int S = diff_parts(tiled, kind, B, heads, pairs, D, max_seq, static_cast<int>(a.num_splits), sm);
+  if (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) ||
+      a.workspace_bytes < diff_rows_bytes(static_cast<int64_t>(S) * B * 2 * heads, D))
     return INT8KV_E_WORKSPACE;
 
   DiffParams d;
   std::memset(&d, 0, sizeof(d));
-  d.heads = a.Hq; d.group = a.Hq / a.Hkv; d.Dk = a.D;
-  d.lam = x.lam; d.lam_dtype = x.lam_dtype; d.lam_st = x.lam_stride;
-  d.norm_w = x.norm_w; d.norm_dtype = x.norm_dtype; d.norm_eps = x.norm_eps; d.out_scale = x.out_scale;
+  d.heads = heads; d.group = heads / pairs; d.Dk = D;
+  d.lam = a.lam; d.lam_dtype = static_cast<int>(a.lam_dtype); d.lam_st = a.lam_stride;
+  d.norm_w = a.norm_weight; d.norm_dtype = static_cast<int>(a.norm_dtype);
+  d.norm_eps = static_cast<float>(a.norm_eps); d.out_scale = static_cast<float>(a.out_scale);
   AttnParams& p = d.a;
-  p.q = a.query; p.q_dtype = a.q_dtype;
-  for (int i = 0; i < 3; ++i) { p.q_st[i] = a.q_st[i]; p.o_st[i] = a.o_st[i]; }
-  p.B = a.B; p.Hq = 2 * a.Hq; p.Hkv = a.Hkv; p.G = 2 * d.group; p.D = 2 * a.D;
-  p.kc = a.kc; p.vc = a.vc; p.cache_kind = a.cache_kind;
-  for (int i = 0; i < 4; ++i) { p.kc_st[i] = a.kc_st[i]; p.vc_st[i] = a.vc_st[i]; }
-  p.num_blocks = a.num_blocks; p.block_size = a.block_size;
-  p.tiles_per_block = a.block_size / 16;
+  p.q = a.query; p.q_dtype = static_cast<int>(a.q_dtype);
+  for (int i = 0; i < 3; ++i) { p.q_st[i] = a.q_strides[i]; p.o_st[i] = a.out_strides[i]; }
+  p.B = B; p.Hq = 2 * heads; p.Hkv = pairs; p.G = 2 * d.group; p.D = 2 * D;
+  p.kc = a.key_cache; p.vc = a.value_cache; p.cache_kind = kind;
+  for (int i = 0; i < 4; ++i) { p.kc_st[i] = a.key_cache_strides[i]; p.vc_st[i] = a.value_cache_strides[i]; }
+  p.num_blocks = a.num_blocks; p.block_size = block_size;
+  p.tiles_per_block = block_size / 16;
   p.hint_tiles = static_cast<int>(tiles);
-  p.bt = a.bt; p.bt_is_i64 = a.bt_is_i64; p.bt_st[0] = a.bt_st[0]; p.bt_st[1] = a.bt_st[1]; p.bt_width = a.bt_width;
-  p.sl = a.sl; p.sl_is_i64 = a.sl_is_i64;
-  p.k_scale = a.k_scale; p.v_scale = a.v_scale;
-  p.out = a.out; p.out_dtype = a.out_dtype;
+  p.bt = a.block_tables; p.bt_is_i64 = a.bt_is_i64 != 0; p.bt_st[0] = a.bt_strides[0]; p.bt_st[1] = a.bt_strides[1];
+  p.bt_width = a.bt_width;
+  p.sl = a.seq_lens; p.sl_is_i64 = a.sl_is_i64 != 0;
+  if (int8_cache) { p.k_scale = a.k_scale; p.v_scale = a.v_scale; }
+  p.out = a.out; p.out_dtype = static_cast<int>(a.out_dtype);
   p.num_splits = S;
   p.per_longest = static_cast<int>(std::max<int64_t>(1, (tiles + S - 1) / S));
-  p.row_floats = partial_row_floats(2 * a.D);
-  p.sm_scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(a.D)));
+  p.row_floats = partial_row_floats(2 * D);
+  p.sm_scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(D)));
   p.status = a.status;
-  p.part = reinterpret_cast<float*>(a.ws);
-  if (!tiled) {
-    const int rc = launch_diff_generic(d, a.stream);
-    return rc != INT8KV_OK ? rc : launch_diff_merge(d, a.stream);
+  p.part = reinterpret_cast<float*>(a.workspace);
+  const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
+  int rc;
+  if (tiled) {
+    alignas(64) CUtensorMap tmK, tmV;
+    auto map = [&](CUtensorMap* m, const void* base, const int64_t* st) {
+      const int64_t pair_st[4] = {st[0], st[1], 2 * st[2], 1};
+      return pair_rows ? make_cache_map(m, base, 1, 128, pairs, a.num_blocks, block_size, pair_st)
+                       : make_cache_map(m, base, esz, D, 2 * pairs, a.num_blocks, block_size, st, 2);
+    };
+    if (!map(&tmK, a.key_cache, a.key_cache_strides) || !map(&tmV, a.value_cache, a.value_cache_strides)) return INT8KV_E_LAUNCH;
+    rc = launch_diff_tiled(d, tmK, tmV, stream);
+  } else {
+    rc = launch_diff_generic(d, stream);
   }
-  alignas(64) CUtensorMap tmK, tmV;
-  auto map = [&](CUtensorMap* m, const void* base, const int64_t* st) {
-    const int64_t pair_st[4] = {st[0], st[1], 2 * st[2], 1};
-    return pair_rows ? make_cache_map(m, base, 1, 128, a.Hkv, a.num_blocks, a.block_size, pair_st)
-                     : make_cache_map(m, base, esz, a.D, 2 * a.Hkv, a.num_blocks, a.block_size, st, 2);
-  };
-  if (!map(&tmK, a.kc, a.kc_st) || !map(&tmV, a.vc, a.vc_st)) return INT8KV_E_LAUNCH;
-  const int rc = launch_diff_tiled(d, tmK, tmV, a.stream);
-  return rc != INT8KV_OK ? rc : launch_diff_merge(d, a.stream);
+  return rc != INT8KV_OK ? rc : launch_diff_merge(d, stream);
 }
 
 }  // namespace
@@ -1230,44 +1215,6 @@ int64_t int8kv_diff_workspace_bytes(int batch, int num_heads, int num_kv_pairs, 
   return diff_rows_bytes(static_cast<int64_t>(parts) * batch * 2 * num_heads, head_dim);
 }
 
-int int8kv_paged_diff_attn_int8(const void* query, int q_dtype, const int64_t q_strides[3], int batch, int num_heads,
-                                int num_kv_pairs, int head_dim, const int8_t* key_cache, const int8_t* value_cache,
-                                const int64_t key_cache_strides[4], const int64_t value_cache_strides[4],
-                                int64_t num_blocks, int block_size, const void* block_tables, int bt_is_i64,
-                                const int64_t bt_strides[2], int64_t bt_width, const void* seq_lens, int sl_is_i64,
-                                int64_t max_seq_len_hint, const float* k_scale, const float* v_scale, const void* lam,
-                                int lam_dtype, int64_t lam_stride, const void* norm_weight, int norm_dtype,
-                                float norm_eps, float out_scale, void* out, int out_dtype, const int64_t out_strides[3],
-                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
-                                void* stream) {
-  AttnCall a{query, q_dtype, q_strides, batch, num_heads, num_kv_pairs, head_dim,
-             key_cache, value_cache, kCacheInt8, key_cache_strides, value_cache_strides, num_blocks, block_size,
-             block_tables, bt_is_i64, bt_strides, bt_width, seq_lens, sl_is_i64, max_seq_len_hint,
-             k_scale, v_scale, out, out_dtype, out_strides, nullptr,
-             num_splits, workspace, workspace_bytes, 0, static_cast<cudaStream_t>(stream)};
-  a.status = status;
-  return run_diff(a, DiffExtra{lam, lam_dtype, lam_stride, norm_weight, norm_dtype, norm_eps, out_scale});
-}
-
-int int8kv_paged_diff_attn_bf16(const void* query, int q_dtype, const int64_t q_strides[3], int batch, int num_heads,
-                                int num_kv_pairs, int head_dim, const void* key_cache, const void* value_cache,
-                                int cache_dtype, const int64_t key_cache_strides[4],
-                                const int64_t value_cache_strides[4], int64_t num_blocks, int block_size,
-                                const void* block_tables, int bt_is_i64, const int64_t bt_strides[2], int64_t bt_width,
-                                const void* seq_lens, int sl_is_i64, int64_t max_seq_len_hint, const void* lam,
-                                int lam_dtype, int64_t lam_stride, const void* norm_weight, int norm_dtype,
-                                float norm_eps, float out_scale, void* out, int out_dtype, const int64_t out_strides[3],
-                                int num_splits, void* workspace, int64_t workspace_bytes, unsigned int* status,
-                                void* stream) {
-  if (cache_dtype != INT8KV_BF16 && cache_dtype != INT8KV_FP16) return INT8KV_E_BAD_DTYPE;
-  AttnCall a{query, q_dtype, q_strides, batch, num_heads, num_kv_pairs, head_dim,
-             key_cache, value_cache, cache_dtype == INT8KV_BF16 ? kCacheBf16 : kCacheFp16,
-             key_cache_strides, value_cache_strides, num_blocks, block_size,
-             block_tables, bt_is_i64, bt_strides, bt_width, seq_lens, sl_is_i64, max_seq_len_hint,
-             nullptr, nullptr, out, out_dtype, out_strides, nullptr,
-             num_splits, workspace, workspace_bytes, 0, static_cast<cudaStream_t>(stream)};
-  a.status = status;
-  return run_diff(a, DiffExtra{lam, lam_dtype, lam_stride, norm_weight, norm_dtype, norm_eps, out_scale});
-}
+int int8kv_paged_diff_attn(const int8kv_diff_args* args) { return args == nullptr ? INT8KV_E_NULLPTR : run_diff(*args); }
 
 }  // extern "C"

@@ -22,9 +22,11 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _FLOAT_CODES, _as_f32_scale, _call, _max_seq_len, _require_lib, _sm_count, _status_ptr
+from .ops import (_FLOAT_CODES, _as_f32_scale, _call, _max_seq_len, _require_lib, _sm_count, _status_ptr,
+                  _stream_ptr)
 
 _INDEX_CODES = {torch.int32: 0, torch.int64: 1}
+_CACHE_CODES = {torch.int8: _lib.INT8, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 
 
 @lru_cache(maxsize=1024)
@@ -77,19 +79,18 @@ def _run(int8, query, key_cache, value_cache, block_tables, seq_lens, k_scale, v
     # The partial rows belong to the call: memory of the current stream, or of the pool of the graph that captures the
     # call.  The status word is the stream's, the one that device_status() reads.
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    i64 = _lib.i64
-    rc = _call(
-        device, lib.int8kv_paged_diff_attn_int8 if int8 else lib.int8kv_paged_diff_attn_bf16,
-        query.data_ptr(), q_code, i64(query.stride()), B, H, P, D, key_cache.data_ptr(), value_cache.data_ptr(),
-        *(() if int8 else (_FLOAT_CODES[key_cache.dtype],)),
-        i64(kc_st), i64(vc_st), num_blocks, block_size, block_tables.data_ptr(), bt_code, i64(bt_st), width,
-        seq_lens.data_ptr(), sl_code, max_seq,
-        *((k_scale.data_ptr(), v_scale.data_ptr()) if int8 else ()),
-        lam.data_ptr(), lam_code, 0 if lams == 1 else lam.stride(0), norm_ptr, norm_code, norm_eps, out_scale,
-        out.data_ptr(), out_code, i64(out.stride()), splits, ws.data_ptr(), nbytes, _status_ptr(device),
+    packed = _lib.DIFF_ARGS.pack(
+        query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+        k_scale.data_ptr() if int8 else 0, v_scale.data_ptr() if int8 else 0, lam.data_ptr(), norm_ptr, out.data_ptr(),
+        ws.data_ptr(), _status_ptr(device), _stream_ptr(device),
+        *query.stride(), *kc_st, *vc_st, *bt_st, *out.stride(),
+        0 if lams == 1 else lam.stride(0), B, H, P, D, num_blocks, block_size, width, max_seq, splits, nbytes,
+        q_code, _CACHE_CODES[key_cache.dtype], lam_code, norm_code, out_code, bt_code, sl_code,
+        norm_eps, out_scale,
     )
+    rc = _call(device, lib.int8kv_paged_diff_attn, packed)
     if rc != _lib.OK:
-        _lib.check("int8kv_paged_diff_attn_int8" if int8 else "int8kv_paged_diff_attn_bf16", rc)
+        _lib.check("int8kv_paged_diff_attn", rc)
     return out
 
 

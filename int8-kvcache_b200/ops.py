@@ -108,12 +108,12 @@ def _status_ptr(device: torch.device) -> int:
     return buf.data_ptr() + ((buf.numel() - 16) & ~15)
 
 
-def _call(device: torch.device, fn, *args) -> int:
-    """fn(*args, current stream of `device`) with `device` current: a launch goes to the device that its stream is of."""
+def _call(device: torch.device, fn, packed: bytes) -> int:
+    """fn(packed) with `device` current: a launch goes to the device that its stream is of."""
     if device.index == torch.cuda.current_device():
-        return fn(*args, _stream_ptr(device))
+        return fn(packed)
     with torch.cuda.device(device):
-        return fn(*args, _stream_ptr(device))
+        return fn(packed)
 
 
 def _as_f32_scale(scale: torch.Tensor) -> torch.Tensor:

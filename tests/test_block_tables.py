@@ -1,8 +1,6 @@
 """Block tables and slot maps without a GPU: the checker against the package's host-side builders, the refusals of
 the Python entry points, and the argument checks of the C ABI."""
 
-import ctypes as C
-
 import pytest
 import torch
 
@@ -41,28 +39,54 @@ def test_c_abi_argument_checks():
     """Null pointers, sizes out of range and a missing workspace are refused before anything is launched."""
     lm = package("_lib")
     lib = lm.load()
-    st = lm.i64((4, 1))
-    p = C.c_void_p(256)  # never dereferenced: every call below is refused
+    p = 256  # never dereferenced: every call below is refused
 
-    def build(R=2, bs=16, width=4, free=8, tokens=4, lens=p, lens_out=p, bt=p, cursor=p, start=p, slots=p, ws=None, ws_bytes=0):
-        return lib.int8kv_build_block_tables(lens, 0, p, 0, R, bs, bt, 0, st, width, p, 0, free, cursor, cursor, lens_out,
-                                             slots, tokens, start, ws, ws_bytes, None)
+    def call(fn, R=2, bs=16, width=4, free=8, tokens=4, lens=p, new=p, done=p, bt=p, cursor=p, start=p, slots=p, fb=p, lens_out=p,
+             ws=0, ws_bytes=0):
+        return fn(lm.TABLE_ARGS.pack(lens, new, done, bt, fb, cursor, cursor, lens_out, slots, start, ws, 0,
+                                     0, 0, 0, 0, R, bs, 4, 1, width, free, tokens, ws_bytes))
 
-    assert build(R=-1) == lm.E_BAD_SHAPE and build(bs=0) == lm.E_BAD_SHAPE and build(width=-1) == lm.E_BAD_SHAPE
-    assert build(tokens=-1) == lm.E_BAD_SHAPE and build(tokens=2**31) == lm.E_BAD_SHAPE
-    assert build(free=-1) == lm.E_BAD_SHAPE and build(width=2**31) == lm.E_BAD_SHAPE
-    assert build(lens=None) == lm.E_NULLPTR and build(bt=None) == lm.E_NULLPTR and build(cursor=None) == lm.E_NULLPTR
-    assert build(start=None) == lm.E_NULLPTR and build(slots=None) == lm.E_NULLPTR
+    build, slot, release = lib.int8kv_build_block_tables, lib.int8kv_build_slot_mapping, lib.int8kv_release_block_tables
+    for fn in (build, slot, release):
+        assert fn(None) == lm.E_NULLPTR
+        assert call(fn, R=-1) == lm.E_BAD_SHAPE and call(fn, R=2**31) == lm.E_BAD_SHAPE
+        assert call(fn, bs=0) == lm.E_BAD_SHAPE and call(fn, bs=2**32 + 16) == lm.E_BAD_SHAPE
+        assert call(fn, width=-1) == lm.E_BAD_SHAPE and call(fn, width=2**31) == lm.E_BAD_SHAPE
+        assert call(fn, lens=0) == lm.E_NULLPTR and call(fn, bt=0) == lm.E_NULLPTR
+    for fn in (build, slot):
+        assert call(fn, tokens=-1) == lm.E_BAD_SHAPE and call(fn, tokens=2**31) == lm.E_BAD_SHAPE
+        assert call(fn, start=0) == lm.E_NULLPTR and call(fn, slots=0) == lm.E_NULLPTR and call(fn, new=0) == lm.E_NULLPTR
+    for fn in (build, release):
+        assert call(fn, free=-1) == lm.E_BAD_SHAPE and call(fn, cursor=0) == lm.E_NULLPTR
+        assert call(fn, fb=0) == lm.E_NULLPTR and call(fn, lens_out=0) == lm.E_NULLPTR
+    assert call(release, done=0) == lm.E_NULLPTR
     big = 1 << 20
     need = lib.int8kv_block_tables_workspace_bytes(2, big + big // 16 + 2, 1)
-    assert need > 0 and build(tokens=big) == lm.E_WORKSPACE
-    assert build(tokens=big, ws=p, ws_bytes=need - 1) == lm.E_WORKSPACE
-    assert build(tokens=big, ws=C.c_void_p(264), ws_bytes=need) == lm.E_WORKSPACE
+    assert need > 0 and call(build, tokens=big) == lm.E_WORKSPACE  # in place: lens_out is lens
+    assert call(build, tokens=big, ws=p, ws_bytes=need - 1) == lm.E_WORKSPACE
+    assert call(build, tokens=big, ws=264, ws_bytes=need) == lm.E_WORKSPACE
     assert lib.int8kv_block_tables_workspace_bytes(64, 128, 1) == 0  # small: one kernel
     assert lib.int8kv_block_tables_workspace_bytes(64, 1 << 20, 0) == 0  # outputs of its own: one kernel of many CTAs
     assert lib.int8kv_block_tables_workspace_bytes(5000, 128, 0) > 0
     assert lib.int8kv_block_tables_workspace_bytes(-1, 128, 0) == -1
-    assert lib.int8kv_build_slot_mapping(p, 0, None, 0, 2, 16, p, 0, st, 4, p, 4, p, None, 0, None) == lm.E_NULLPTR
-    assert lib.int8kv_build_slot_mapping(p, 0, p, 0, 2, 0, p, 0, st, 4, p, 4, p, None, 0, None) == lm.E_BAD_SHAPE
-    assert lib.int8kv_release_block_tables(p, 0, None, 2, 16, p, 0, st, 4, p, 0, 8, p, p, p, None, 0, None) == lm.E_NULLPTR
-    assert lib.int8kv_release_block_tables(p, 0, p, 2, 16, p, 0, st, 4, None, 0, 8, p, p, p, None, 0, None) == lm.E_NULLPTR
+
+
+def test_argument_records_have_the_size_of_the_structs(tmp_path):
+    """The flat records that the binding packs are the structs of the header."""
+    import shutil
+    import subprocess
+
+    from conftest import REPO
+
+    lm = package("_lib")
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "int8kv_b200.h"\nint main(void) {\n'
+                   'printf("%zu %zu %zu %zu %zu\\n", sizeof(int8kv_diff_args), sizeof(int8kv_table_args),'
+                   ' offsetof(int8kv_diff_args, lam_stride), offsetof(int8kv_diff_args, norm_eps),'
+                   ' offsetof(int8kv_table_args, num_requests)); return 0; }\n')
+    subprocess.run([gcc, "-I", str(REPO / "include"), str(src), "-o", str(tmp_path / "sizes")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [lm.DIFF_ARGS.size, lm.TABLE_ARGS.size, 8 * 29, 8 * 47, 8 * 16]

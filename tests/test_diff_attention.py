@@ -1,8 +1,6 @@
 """Differential attention without a GPU: the checker against the elementary formula, refusals of host tensors, and the
 argument checks of the C ABI."""
 
-import ctypes as C
-
 import pytest
 import torch
 
@@ -40,28 +38,25 @@ def test_entry_points_refuse_host_tensors(kv):
 def test_c_abi_argument_checks():
     lm = package("_lib")
     lib = lm.load()
-    p = C.c_void_p(256)  # never dereferenced: every call below is refused
-    s3, s4, s2 = lm.i64((512, 128, 1)), lm.i64((8192, 512, 128, 1)), lm.i64((4, 1))
+    p = 256  # never dereferenced: every call below is refused or empty
 
-    def call(B=2, H=4, P=2, D=128, bs=16, q=p, lam=p, ks=p, qd=lm.BF16, ld=lm.FP32, norm=None, eps=1e-5, splits=1, ws=p,
-             ws_bytes=1 << 20, st=s4, out=p):
-        return lib.int8kv_paged_diff_attn_int8(q, qd, s3, B, H, P, D, p, p, st, st, 4, bs, p, 0, s2, 4, p, 0, 64, ks, p,
-                                               lam, ld, 1, norm, lm.FP32, eps, 1.0, out, lm.BF16, s3, splits, ws, ws_bytes,
-                                               None, None)
+    def call(B=2, H=4, P=2, D=128, bs=16, width=4, q=p, lam=p, ks=p, out=p, qd=lm.BF16, cd=lm.INT8, ld=lm.FP32, norm=0, eps=1e-5,
+             splits=1, ws=p, ws_bytes=1 << 20, last=1):
+        return lib.int8kv_paged_diff_attn(lm.DIFF_ARGS.pack(
+            q, p, p, p, p, ks, p, lam, norm, out, ws, 0, 0, 512, 128, 1, 8192, 512, 128, last, 8192, 512, 128, last, width, 1, 1024,
+            256, 1, 1, B, H, P, D, 4, bs, width, 64, splits, ws_bytes, qd, cd, ld, lm.FP32, lm.BF16, 0, 0, eps, 1.0))
 
+    assert lib.int8kv_paged_diff_attn(None) == lm.E_NULLPTR
     assert call(B=0) == lm.OK
     assert call(B=-1) == lm.E_BAD_SHAPE and call(H=3) == lm.E_BAD_SHAPE and call(P=0) == lm.E_BAD_SHAPE
-    assert call(bs=0) == lm.E_BAD_SHAPE and call(splits=-1) == lm.E_BAD_SHAPE and call(splits=1000) == lm.E_BAD_SHAPE
-    assert call(qd=7) == lm.E_BAD_DTYPE and call(ld=-1) == lm.E_BAD_DTYPE
+    assert call(bs=0) == lm.E_BAD_SHAPE and call(bs=2**32 + 16) == lm.E_BAD_SHAPE and call(B=2**31) == lm.E_BAD_SHAPE
+    assert call(splits=-1) == lm.E_BAD_SHAPE and call(splits=1000) == lm.E_BAD_SHAPE and call(width=-1) == lm.E_BAD_SHAPE
+    assert call(qd=lm.INT8) == lm.E_BAD_DTYPE and call(ld=-1) == lm.E_BAD_DTYPE and call(cd=lm.FP32) == lm.E_BAD_DTYPE
     assert call(norm=p, eps=0.0) == lm.E_BAD_SHAPE and call(norm=p, eps=float("nan")) == lm.E_BAD_SHAPE
-    assert call(D=257) == lm.E_UNSUPPORTED and call(st=lm.i64((8192, 512, 128, 2))) == lm.E_UNSUPPORTED
+    assert call(D=257) == lm.E_UNSUPPORTED and call(last=2) == lm.E_UNSUPPORTED and call(H=65536, P=1) == lm.E_UNSUPPORTED
     for missing in ("q", "lam", "ks", "out"):
-        assert call(**{missing: None}) == lm.E_NULLPTR
+        assert call(**{missing: 0}) == lm.E_NULLPTR
     need = lib.int8kv_diff_workspace_bytes(2, 4, 2, 128, 64, 16, 1, 148)
     assert need == 2 * 8 * 260 * 4
-    assert call(ws=None) == lm.E_WORKSPACE and call(ws_bytes=need - 1) == lm.E_WORKSPACE
-    assert call(ws=C.c_void_p(264)) == lm.E_WORKSPACE
+    assert call(ws=0) == lm.E_WORKSPACE and call(ws_bytes=need - 1) == lm.E_WORKSPACE and call(ws=264) == lm.E_WORKSPACE
     assert lib.int8kv_diff_workspace_bytes(2, 3, 2, 128, 64, 16, 1, 148) == -1
-    assert lib.int8kv_paged_diff_attn_bf16(p, lm.BF16, s3, 2, 4, 2, 128, p, p, lm.FP32, s4, s4, 4, 16, p, 0, s2, 4, p, 0,
-                                           64, p, lm.FP32, 1, None, 0, 1e-5, 1.0, p, lm.BF16, s3, 1, p, 1 << 20, None,
-                                           None) == lm.E_BAD_DTYPE
