@@ -509,13 +509,14 @@ __device__ __forceinline__ void diff_scores(int (&s)[NB][4], uint32_t kb, const 
 // Items resident per SM and ring depth: 192 KB of ring per SM (the bytes in flight that keep HBM busy); a stage is 8 KB
 // for D = 128 and 4 KB for D = 64.  kTrip tiles are consumed per trip: with 4 KB tiles two, for which one softmax step
 // serves both.  The accumulators, 32 floats per lane and (column block, 128 values of V), set how many warps the register
-// file carries.
+// file carries; more, shallower rings win as long as two trips fit (61 ragged sequences of up to 8191 tokens, D = 64, no
+// groups: 12 / 16 per SM 87.6 / 85.4 us; 16 x 4096, D = 128, groups of four: 8 / 10 per SM 20.0 / 22.0 us).
 template <int DK, int NB>
 struct DiffInt8Shape {
   static constexpr int kHalves = DK / 64;
   static constexpr int kStage = kHalves * 4096;
   static constexpr int kTrip = DK == 128 ? 1 : 2;
-  static constexpr int kPerSm = DK == 64 && NB == 1 ? 12 : 8;
+  static constexpr int kPerSm = DK == 64 && NB == 1 ? 16 : 8;
   static constexpr int kStages = 192 * 1024 / (kPerSm * kStage);
   static constexpr int kSmem = kStages * (kStage + 8) + 1024;
 };
@@ -714,10 +715,12 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 // ---------------------------------------------------------------------------------------------
 // bf16 / fp16 caches: same ring and columns, fragments straight from shared memory with ldmatrix
 // ---------------------------------------------------------------------------------------------
+// A stage is 16 KB for D = 128 and 8 KB for D = 64 (45 ragged fp16 sequences of up to 8191 tokens, D = 128, groups of four:
+// 4 items of 3 stages / 6 of 2 per SM 120 / 115 us).
 template <int DK>
 struct DiffF16Shape {
   static constexpr int kStage = DK * 128;  // 2 tensors x 2 heads x 16 tokens x 2 DK bytes
-  static constexpr int kPerSm = DK == 128 ? 4 : 8;
+  static constexpr int kPerSm = DK == 128 ? 6 : 12;
   static constexpr int kStages = 192 * 1024 / (kPerSm * kStage);
   static constexpr int kSmem = kStages * (kStage + 8) + 1024;
 };
