@@ -185,21 +185,24 @@ __device__ __forceinline__ int col_map(int nb, int c) { return NB == 1 ? c >> 2 
 template <int NB>
 __device__ __forceinline__ int col_pair(int c) { return NB == 1 ? c & 3 : c; }
 
-// Running softmax of the columns of one block: reference m of columns 2t (index 0) and 2t+1, in log2 units.  It is a score
-// that was the column's maximum when it was set, and follows the maximum only when that has moved more than SLACK above
-// it: probabilities reach up to 2^SLACK, which the 16-bit P and the fp32 sums hold with the same relative precision as
-// values up to 1.  A step then needs no reduction across the token lanes, just a vote, and with SLACK = 8 the accumulators
-// are rescaled a few times per part instead of in every other tile (INT8, 32 x 32k tokens, groups of eight: 324 -> 309
-// us).  SLACK = 0 keeps the largest probability at 1, which is exact however few bits P has: of use where P has the 8 bits
-// of bf16 (8 x 4096 tokens: error against 64 bits 0.0019 of the output's norm instead of 0.0023, of which the output's own
-// rounding is 0.0017; 22.1 us instead of 21.8).
-
-// One online-softmax step over NV / 2 score rows per lane and NB column blocks at once.  x: scores before the factors
-// sc, x[nb][2k] and x[nb][2k+1] being columns 2t and 2t+1 of token row g + 8k, of which the first `valid` count.  x becomes
-// the probabilities 2^(x sc - m); returns whether m moved, and with it the accumulators, by f[nb][0], f[nb][1].
+// Running softmax of the columns of one block: reference m of columns 2t (index 0) and 2t+1, in log2 units, p =
+// 2^(score - m).  m is set to OFFSET below a column's maximum, so that the maximum has p = 2^OFFSET, and is set again only
+// when a score reaches more than SLACK above that maximum.
+//  * OFFSET + SLACK = 15 keeps p inside fp16 (65504) and uses its range: what fp16 P loses starts 2^-32 below the maximum,
+//    not 2^-25, which a crowd of many tokens far below one that dominates would feel.
+//  * A step needs no reduction across the token lanes, just a vote, and with SLACK = 8 the accumulators are rescaled a few
+//    times per part instead of in every other tile (INT8, 32 x 32k tokens, groups of eight: 324 -> 309 us).
+//  * SLACK = 0 keeps the largest probability a power of two, which is exact however few bits P has: of use where P has
+//    the 8 bits of bf16 (8 x 4096 tokens: error against 64 bits 0.0019 of the output's norm instead of 0.0023, of which the
+//    output's own rounding is 0.0017; 22.1 us instead of 21.8).
+//
+// One step over NV / 2 score rows per lane and NB column blocks at once.  x: scores before the factors sc, x[nb][2k] and
+// x[nb][2k+1] being columns 2t and 2t+1 of token row g + 8k, of which the first `valid` count.  x becomes the
+// probabilities; returns whether m moved, and with it the accumulators, by f[nb][0], f[nb][1].
 template <int SLACK, int NB, int NV>
 __device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][NV], const float (&sc)[NB][2], float (&f)[NB][2],
                                              int valid, int g) {
+  constexpr float kTop = 15.f, kOffset = kTop - SLACK;
   float y[NB][NV];
   float top = -INFINITY;
 #pragma unroll
@@ -218,7 +221,7 @@ __device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][N
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int k = 0; k < NV; ++k) top = fmaxf(top, y[nb][k]);
-  const bool moved = __any_sync(kFull, top > static_cast<float>(SLACK));  // also while m is -inf: y is +inf then
+  const bool moved = __any_sync(kFull, top > kTop);  // also while m is -inf: y is +inf then
   if (moved) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -233,7 +236,7 @@ __device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][N
         z = fmaxf(z, __shfl_xor_sync(kFull, z, 4));
         z = fmaxf(z, __shfl_xor_sync(kFull, z, 8));
         z = fmaxf(z, __shfl_xor_sync(kFull, z, 16));
-        z = fmaxf(z, m[nb][e]);
+        z = fmaxf(z - kOffset, m[nb][e]);
         f[nb][e] = z == m[nb][e] ? 1.f : exp2_fast(m[nb][e] - z);  // equal also when nothing but -inf was seen
         m[nb][e] = z;
 #pragma unroll

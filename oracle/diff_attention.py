@@ -18,7 +18,9 @@ def diff_paged_attention(query, key_cache, value_cache, block_tables, seq_lens, 
     relative for fp16, 2^-8 for a bf16 cache), in the product and in the sum it is divided by alike.  A score moves by at
     most ds = max_n sum_d |dq_d k_nd| / sqrt(D); with it every weight by a factor within exp(+-ds), numerator and
     denominator both, and a map's output by 2 ds sum_n p_n |v_n|.  Rounded weights p (1 + e), |e| <= dp, move
-    o = sum p v / sum p by at most dp sum p |v - o| <= 2 dp sum p |v| (normalised p).  fp32 sums, exponentials and
+    o = sum p v / sum p by at most dp sum p |v - o| <= 2 dp sum p |v| (normalised p).  Where fp16 runs out of
+    exponents, 2^-32 below the largest probability, a weight is off by at most that much, which moves o by at most
+    2^-32 sum (|v| + |o|).  fp32 sums, exponentials and
     divisions add less than 2^-14 of the same.  The norm divides by the row's root mean square r and moves with it, which at most doubles
     a relative error.
     """
@@ -51,6 +53,7 @@ def diff_paged_attention(query, key_cache, value_cache, block_tables, seq_lens, 
                 ds = float((k[:, 2 * g + m].abs() @ dq).amax()) / math.sqrt(D)
                 f = 1.0 if m == 0 else float(lam[h])
                 out[b, h] += (1.0 if m == 0 else -1.0) * f * (p @ v[:, g])
+                bound[b, h] += abs(f) * 2.0 ** -32 * (v[:, g].abs().sum(0) + n * (p @ v[:, g]).abs())
                 bound[b, h] += abs(f) * math.exp(2 * ds) * (2 * ds + 2 * dp + 2.0 ** -14) * (p @ v[:, g].abs())
     bound *= abs(out_scale)
     scaled = out * out_scale
