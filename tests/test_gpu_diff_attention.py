@@ -188,6 +188,28 @@ def test_bad_values_stay_in_their_head(kv):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("cache", [torch.int8, torch.float16], ids=["int8", "fp16"])
+@pytest.mark.parametrize("D", [128, 64])
+def test_a_crowd_far_below_one_token(kv, cache, D):
+    """20000 tokens, each 2^-27 of a token that dominates but has no value: together they are the whole output, and each
+    of them is below what fp16 holds next to 1."""
+    n, bs = 20000, 16
+    c = make_case(30, [n], 2, 1, D, bs, cache)
+    first = c["bt"][0, 0].item()
+    c["kc"].zero_()
+    c["kc"][first, 0] = 100 if cache == torch.int8 else 2.0
+    c["vc"].fill_(100 if cache == torch.int8 else 1.0)
+    c["vc"][first, 0] = 0
+    if cache == torch.int8:
+        c["ks"].fill_(0.02)
+        c["vs"].fill_(0.01)
+    c["q"].fill_(27 / 2.0 / D ** 0.5 / 1.4426950408889634)
+    c["lam"].fill_(0.25)
+    out = torch.empty(1, 2, 2 * D, dtype=torch.float32, device=DEV)
+    got = verify(kv, c, out=out)
+    assert (got > 0.75 * 0.9 * n * 2.0 ** -27).all()
+
+
 def test_equal_maps_cancel(kv):
     """The same queries and keys in both maps and lam = 1: what is left is rounding, whatever the length."""
     for D in (128, 64):
