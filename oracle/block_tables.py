@@ -1,4 +1,4 @@
-"""Block tables and slot maps, request by request in Python integers: the checker of the device operators."""
+"""Block tables and slot maps, request by request in Python integers: the oracle of the device operators."""
 
 from __future__ import annotations
 

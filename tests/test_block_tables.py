@@ -1,4 +1,4 @@
-"""Block tables and slot maps without a GPU: the checker against the package's host-side builders, the refusals of
+"""Block tables and slot maps without a GPU: the oracle against the package's host-side builders, the refusals of
 the Python entry points, and the argument checks of the C ABI."""
 
 import pytest
@@ -8,7 +8,7 @@ from conftest import package
 from oracle import block_tables as oracle_tables
 
 
-def test_checker_agrees_with_the_host_side_builders(workloads):
+def test_oracle_agrees_with_the_host_side_builders(workloads):
     """Tables grown from nothing out of a permuted pool are the tables and slots that the workloads build on the host."""
     lens = [17, 1, 0, 64, 33]
     need = workloads.blocks_needed(lens, 16)

@@ -1,4 +1,4 @@
-"""Differential attention without a GPU: the checker against the elementary formula, refusals of host tensors, and the
+"""Differential attention without a GPU: the oracle against the elementary formula, refusals of host tensors, and the
 argument checks of the C ABI."""
 
 import pytest
@@ -8,8 +8,8 @@ from conftest import package
 from oracle.diff_attention import diff_paged_attention
 
 
-def test_checker_is_the_difference_of_two_ordinary_attentions():
-    """Against the fp32 checker of ordinary decode attention, run once per map and half of V."""
+def test_oracle_is_the_difference_of_two_ordinary_attentions():
+    """Against the fp32 oracle of ordinary decode attention, run once per map and half of V."""
     import oracle
 
     torch.manual_seed(0)

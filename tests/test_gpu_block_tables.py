@@ -1,4 +1,4 @@
-"""Block tables and slot maps on the GPU against the request-by-request checker: every value is an integer and has
+"""Block tables and slot maps on the GPU against the request-by-request oracle: every value is an integer and has
 to be equal."""
 
 import random
@@ -51,7 +51,7 @@ CASES = [  # requests, width, block size, lo, hi, new_hi, spare
 @pytest.mark.parametrize("case", CASES, ids=str)
 @pytest.mark.parametrize("types", [(torch.int32, torch.int32), (torch.int64, torch.int64), (torch.int32, torch.int64)],
                          ids=["i32", "i64", "mixed"])
-def test_build_and_release_match_the_checker(kv, case, types):
+def test_build_and_release_match_the_oracle(kv, case, types):
     requests, width, bs, lo, hi, new_hi, spare = case
     table, lens, new, pool, cursor = make_state(hash(case) & 0xffff, requests, width, bs, lo, hi, new_hi, spare, *types)
     total = int(new.sum())
@@ -179,7 +179,7 @@ def test_refusals(kv):
 
 @pytest.mark.parametrize("requests,prompt", [(37, 0), (9, 12000)], ids=["one_kernel", "two_kernels"])
 def test_captured_step_advances_its_own_state(kv, requests, prompt):
-    """Lengths and cursor in place, captured once: every replay is one more step of the checker."""
+    """Lengths and cursor in place, captured once: every replay is one more step of the oracle."""
     table, lens, new, pool, cursor = make_state(11, requests, 900, 16, 0, 90, 1, 64 * 16 + 8 * prompt)
     new[:] = 1
     new[requests // 2] = max(1, prompt)
