@@ -22,8 +22,9 @@
 namespace int8kv {
 
 
-// The m of a partial row: a column of nothing but NaN has no reference (m = -inf) and must not pass for an empty part.
-__device__ __forceinline__ float part_ref(float m, float l) { return l != l ? l : m; }
+// Reference of a softmax that has seen no score.  Finite, so that a score of -inf (a token that a -inf in its key masks)
+// gives p = 0 even ahead of the first finite one, and a part of nothing but such tokens, or of NaN, is no empty part.
+constexpr float kNoRef = -3.402823466e38f;
 
 // ---------------------------------------------------------------------------------------------
 // Every shape: one warp per (sequence, query pair, split), lanes over the dims, four tokens per step, plain loads.
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(128) diff_generic_kernel(const DiffParams d) {
       q[m][s] = dd < D ? load_as_float(p.q, p.q_dtype, b * p.q_st[0] + (2 * h + m) * p.q_st[1] + dd * p.q_st[2]) : 0.f;
       acc[m][0][s] = acc[m][1][s] = 0.f;
     }
-  float ksc[2], mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float ksc[2], mx[2] = {kNoRef, kNoRef}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     ksc[m] = (p.k_scale ? fmaxf(__ldg(p.k_scale + 2 * pair + m), 1e-6f) : 1.f) * p.sm_scale_log2;
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(128) diff_generic_kernel(const DiffParams d) {
         dot[u] = ok[u] ? dot[u] * ksc[m] : -INFINITY;
         mn = fmaxf(mn, dot[u]);
       }
-      const float al = mx[m] == -INFINITY ? 0.f : exp2f(mx[m] - mn);
+      const float al = exp2f(mx[m] - mn);
       float sum = 0.f;
 #pragma unroll
       for (int u = 0; u < kTok; ++u) {
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(128) diff_generic_kernel(const DiffParams d) {
         if (dd < D) out[half * D + dd] = acc[m][half][s];
       }
     if (lane == 0) {
-      out[p.D] = part_ref(mx[m], l[m]);
+      out[p.D] = mx[m];
       out[p.D + 1] = l[m];
     }
   }
@@ -221,7 +222,7 @@ __device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][N
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int k = 0; k < NV; ++k) top = fmaxf(top, y[nb][k]);
-  const bool moved = __any_sync(kFull, top > kTop);  // also while m is -inf: y is +inf then
+  const bool moved = __any_sync(kFull, top > kTop);  // also while m is kNoRef: y is huge then
   if (moved) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -237,7 +238,7 @@ __device__ __forceinline__ bool softmax_step(float (&m)[NB][2], float (&x)[NB][N
         z = fmaxf(z, __shfl_xor_sync(kFull, z, 8));
         z = fmaxf(z, __shfl_xor_sync(kFull, z, 16));
         z = fmaxf(z - kOffset, m[nb][e]);
-        f[nb][e] = z == m[nb][e] ? 1.f : exp2_fast(m[nb][e] - z);  // equal also when nothing but -inf was seen
+        f[nb][e] = z == m[nb][e] ? 1.f : exp2_fast(m[nb][e] - z);  // 0 for the first score: kNoRef is that far below
         m[nb][e] = z;
 #pragma unroll
         for (int k = e; k < NV; k += 2) y[nb][k] -= z;
@@ -643,7 +644,7 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
   float acc[HV][NB][8][4], sum[NB][4], m[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    m[nb][0] = m[nb][1] = -INFINITY;
+    m[nb][0] = m[nb][1] = kNoRef;
     sum[nb][0] = sum[nb][1] = sum[nb][2] = sum[nb][3] = 0.f;
 #pragma unroll
     for (int h = 0; h < HV; ++h)
@@ -710,7 +711,7 @@ diff_int8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
       for (int h = 0; h < HV; ++h)
 #pragma unroll
         for (int j = 0; j < 8; ++j) sts64(row + (128 * h + 16 * j + 2 * g) * 4, acc[h][nb][j][e], acc[h][nb][j][e + 2]);
-      if (g == 0) sts128(row + 2 * DK * 4, part_ref(m[nb][e], sum[nb][e]), sum[nb][e], 0.f, 0.f);
+      if (g == 0) sts128(row + 2 * DK * 4, m[nb][e], sum[nb][e], 0.f, 0.f);
     }
   store_rows<NB, 2 * DK>(prow, ring.stage0, d.group, lane);
 }
@@ -785,7 +786,7 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   float acc[2][NB][STEPS][4], sum[NB][4], m[NB][2], sc[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    m[nb][0] = m[nb][1] = -INFINITY;
+    m[nb][0] = m[nb][1] = kNoRef;
     sc[nb][0] = sc[nb][1] = p.sm_scale_log2;
     sum[nb][0] = sum[nb][1] = sum[nb][2] = sum[nb][3] = 0.f;
 #pragma unroll
@@ -881,7 +882,7 @@ diff_f16_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
           sts32(row + (DK * h + 16 * j + g) * 4, acc[h][nb][j][e]);
           sts32(row + (DK * h + 16 * j + g + 8) * 4, acc[h][nb][j][e + 2]);
         }
-      if (g == 0) sts128(row + 2 * DK * 4, part_ref(m[nb][e], sum[nb][e]), sum[nb][e], 0.f, 0.f);
+      if (g == 0) sts128(row + 2 * DK * 4, m[nb][e], sum[nb][e], 0.f, 0.f);
     }
   store_rows<NB, 2 * DK>(prow, ring.stage0, d.group, lane);
 }

@@ -141,7 +141,8 @@ def bf16_paged_diff_attention(
     max_seq_len: Optional[int] = None,
     out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """The same over a bf16 or fp16 paged cache, the same-run baseline of the INT8 form."""
+    """The same over a bf16 or fp16 paged cache, the same-run baseline of the INT8 form.  The query is rounded to the
+    caches' type, so with fp16 caches it has to lie in fp16's range.  A key that makes a token's scores -inf masks it."""
     assert key_cache.dtype in (torch.bfloat16, torch.float16) and value_cache.dtype == key_cache.dtype
     return _run(False, query, key_cache, value_cache, block_tables, seq_lens, None, None, lam, norm_weight, norm_eps,
                 out_scale, num_splits, max_seq_len, out)

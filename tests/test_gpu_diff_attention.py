@@ -188,6 +188,28 @@ def test_bad_values_stay_in_their_head(kv):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("cache", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("D", [128, 64, 48])
+@pytest.mark.parametrize("heads", [4, 14])
+def test_tokens_masked_by_an_infinite_key(kv, cache, D, heads):
+    """A first block whose scores are -inf is as if it were not there; a sequence of nothing else attends to
+    nothing."""
+    c = make_case(23, [96, 33], heads, 2, D, 16, cache)
+    c["q"][..., 0] = c["q"][..., 0].abs() + 0.5
+    out = lambda: torch.empty(2, heads, 2 * D, dtype=torch.float32, device=DEV)
+    rest = dict(c, bt=c["bt"][:, 1:].contiguous(), lens=c["lens"] - 16)
+    kc = c["kc"].clone()
+    kc[c["bt"][:, 0].long(), :, :, 0] = float("-inf")
+    # one part: the masked block leaves sums of 0, and what follows is the same arithmetic
+    assert torch.equal(call(kv, dict(c, kc=kc), num_splits=1, out=out()), call(kv, rest, num_splits=1, out=out()))
+    # a block per part: the join adds the same six values in another order, each addition off by 2^-24 of sum p |v|
+    a, b = call(kv, dict(c, kc=kc), num_splits=6, out=out()), call(kv, rest, num_splits=5, out=out())
+    room = 16 * 2.0 ** -24 * c["vc"].float().abs().max().item() * (1 + c["lam"].abs().max().item())
+    assert (a - b).abs().max().item() <= room
+    kc[..., 0] = float("-inf")
+    assert (call(kv, dict(c, kc=kc)) == 0).all()
+
+
 @pytest.mark.parametrize("cache", [torch.int8, torch.float16], ids=["int8", "fp16"])
 @pytest.mark.parametrize("D", [128, 64])
 def test_a_crowd_far_below_one_token(kv, cache, D):
